@@ -280,6 +280,17 @@ int32_t wgf_tensor_llama_block(wgf_tensor* x, wgf_tensor* const* weights, wgf_te
                                wgf_tensor* cos, wgf_tensor* sin, wgf_tensor* mask, uint32_t n_heads, float eps,
                                wgf_tensor** out);
 
+/* Norm and rotation of queries and keys, lazily, as ONE kernel (no counterpart in the crate):
+ *   y = x / sqrt(mean(x^2) + eps) * weight over each head's head_dim values, then
+ *   out[d] = y[d] cos[p][d] - y[d + D/2] sin[p][d], out[d + D/2] = y[d + D/2] cos[p][d] + y[d] sin[p][d],
+ * with p = start + the token's index.  q and k are [heads, seq, head_dim] or [batch, heads, seq, head_dim]
+ * (any strides: a transposed view of a projection costs nothing) and may differ in their heads alone;
+ * q_weight, k_weight [head_dim]; cos / sin [>= start + seq, head_dim / 2]; all of one element type.
+ * head_dim is even and at most 512.  Everything is computed in f32 and rounded once (unlike
+ * wgf_tensor_layer_norm and wgf_tensor_rope, which round after every step as the crate does). */
+int32_t wgf_tensor_qk_norm_rope(wgf_tensor* q, wgf_tensor* k, wgf_tensor* q_weight, wgf_tensor* k_weight, wgf_tensor* cos,
+                                wgf_tensor* sin, float eps, int64_t start, wgf_tensor** q_out, wgf_tensor** k_out);
+
 /* LazyTensorData::materialize, src/tensor.rs:286-288: resolves the graph below `t`
  * (src/compute_graph/resolve.rs:16-248) and queues its kernels; does not wait. */
 int32_t wgf_tensor_materialize(wgf_tensor* t);
@@ -307,6 +318,76 @@ int32_t wgf_tensor_timing_labels(wgf_tensor* t, char* dst, uint64_t capacity, ui
 int32_t wgf_tensor_graphviz(wgf_tensor* t, char* dst, uint64_t capacity, uint64_t* needed);
 /* Number of live graph nodes reachable from the graph `t` belongs to (debug aid). */
 int32_t wgf_tensor_graph_size(wgf_tensor* t, uint64_t* nodes);
+
+/* ======================================================================================
+ * Decoding token by token (no counterpart in the crate): an 8-bit key/value cache with the
+ * attention that reads it, and products with 4-bit weights.
+ *
+ * A cache holds `batch` sequences of up to `capacity` tokens.  Each block of 64 tokens of one
+ * kv head has one scale for its keys and one for its values: scale = max|x| / 127, code =
+ * 127 x / max|x| rounded to the nearest, ties to even (max|x| is taken as 2^-100 at least; a
+ * block with a value that is not finite gets a NaN scale, which reaches every query that sees
+ * the block).  The block that is still open is coded anew, from its tokens' own values, with
+ * every append: what the cache holds depends on the tokens and not on the calls that brought
+ * them.  Cache calls run at once, in the order in which they are made (a lazy operand is
+ * materialised first); they take tensors of the cache's element type, of any strides.
+ * Appends may be recorded in a schedule: every launch then appends again, and a launch that
+ * would not fit is refused.  Creating, truncating and reading, and explicit `counts`, cannot
+ * be recorded (WGF_ERR_UNSUPPORTED).
+ * ==================================================================================== */
+typedef struct wgf_kv_cache wgf_kv_cache;
+/* head_dim: a multiple of 8, at most 256. */
+int32_t wgf_kv_cache_create(wgf_device* dev, uint32_t dtype, int64_t batch, int64_t kv_heads, int64_t head_dim, int64_t capacity,
+                            wgf_kv_cache** out);
+int32_t wgf_kv_cache_retain(wgf_kv_cache* cache);
+int32_t wgf_kv_cache_release(wgf_kv_cache* cache);
+/* Tokens of each sequence, `batch` numbers. */
+int32_t wgf_kv_cache_lengths(wgf_kv_cache* cache, int64_t* lengths);
+/* Takes tokens back (drafts that were not accepted) or empties sequences: `batch` new lengths, none
+ * above the present one.  The tokens of the open block and of the one before it are still held in
+ * the element type, so at least the last 64 can go; further back a length must be a multiple of 64
+ * (WGF_ERR_UNSUPPORTED otherwise, and nothing is changed). */
+int32_t wgf_kv_cache_truncate(wgf_kv_cache* cache, const int64_t* lengths);
+/* k, v [batch, kv_heads, tokens, head_dim] behind each sequence's last token.  `counts` (NULL: all)
+ * says how many of the tokens each sequence takes, from the first on; the rest is padding and not
+ * read.  WGF_ERR_INVALID_ARGUMENT, and nothing is changed, if a sequence would not fit. */
+int32_t wgf_kv_cache_append(wgf_kv_cache* cache, wgf_tensor* k, wgf_tensor* v, const int64_t* counts);
+/* wgf_tensor_qk_norm_rope and wgf_kv_cache_append in one launch, with every sequence's tokens at its own
+ * positions (its length on): q [batch, heads, tokens, head_dim] comes back normed and rotated, k goes to
+ * the cache.  cos / sin reach to the longest sequence's last new token.  Rows of q behind a sequence's
+ * count come back as zeros. */
+int32_t wgf_kv_cache_append_qk(wgf_kv_cache* cache, wgf_tensor* q, wgf_tensor* k, wgf_tensor* v, wgf_tensor* q_weight,
+                               wgf_tensor* k_weight, wgf_tensor* cos, wgf_tensor* sin, float eps, const int64_t* counts,
+                               wgf_tensor** q_out);
+/* softmax(scale * q K^T) V for q [batch, heads, tokens, head_dim], heads a multiple of kv_heads (query
+ * head h reads kv head h * kv_heads / heads).  The queries stand at the last positions of their sequence
+ * (with `counts`, the first counts[b] of them do and the others are padding) and each sees the tokens up
+ * to its own.  A query before the sequence's first token, and a padding one, gives zeros.  Made for a
+ * few tokens a sequence; scores, sums and products are f32 for every element type. */
+int32_t wgf_kv_cache_attention(wgf_kv_cache* cache, wgf_tensor* q, float scale, const int64_t* counts, wgf_tensor** out);
+/* The values that the codes stand for: two tensors [batch, kv_heads, longest length, head_dim], zero
+ * behind each sequence's end. */
+int32_t wgf_kv_cache_read(wgf_kv_cache* cache, wgf_tensor** k, wgf_tensor** v);
+
+/* 4-bit weights [n, k]: value = scale * (code - 8), code 0..15, one scale for each row and `group`
+ * (32, 64 or 128) columns; the last group of a row may be short. */
+typedef struct wgf_q4_weight wgf_q4_weight;
+/* From a [n, k] tensor: scale = max|w| * (1/7) as a product in f32, rounded to the tensor's type; code =
+ * w / scale rounded to the nearest (ties to even) + 8.  A group with a value that is not finite gets a NaN scale. */
+int32_t wgf_q4_weight_quantize(wgf_tensor* w, uint32_t group, wgf_q4_weight** out);
+/* From codes that exist: `codes` [n][(k + 1) / 2] bytes, the even column in the low half; `scales`
+ * [n][(k + group - 1) / group] of `scale_dtype`. */
+int32_t wgf_q4_weight_from_host(wgf_device* dev, int64_t n, int64_t k, uint32_t group, const uint8_t* codes, uint32_t scale_dtype,
+                                const void* scales, wgf_q4_weight** out);
+int32_t wgf_q4_weight_retain(wgf_q4_weight* w);
+int32_t wgf_q4_weight_release(wgf_q4_weight* w);
+int32_t wgf_q4_weight_info(wgf_q4_weight* w, int64_t* n, int64_t* k, uint32_t* group, uint32_t* scale_dtype);
+/* The values as a [n, k] tensor of `dtype`. */
+int32_t wgf_q4_weight_dequantize(wgf_q4_weight* w, uint32_t dtype, wgf_tensor** out);
+/* x [.., k] times the transposed weights: [.., n] of x's type, lazily.  A few rows are one kernel that
+ * reads the codes, with f32 sums of exact products; for many rows the weights are first written
+ * out in x's type (their values rounded to it) and the matrix product runs on them. */
+int32_t wgf_tensor_matmul_q4(wgf_tensor* x, wgf_q4_weight* w, wgf_tensor** out);
 
 /* ======================================================================================
  * Multi-GPU (no counterpart in the crate, which drives one device): one process per GPU;

@@ -101,6 +101,100 @@ class Schedule {
     bool recording_ = true;
 };
 
+template <int R, typename D> class Tensor;
+
+// 4-bit weights [n, k] with group scales (wgf_q4_weight_*); copies are handles on the same weights.
+class Q4Weight {
+   public:
+    explicit Q4Weight(wgf_q4_weight* raw) : h_(raw) {}
+    // codes [n][(k + 1) / 2], the even column in the low half of a byte; scales [n][(k + group - 1) / group]
+    template <typename S>
+    static Q4Weight from_codes(const Device& dev, int64_t n, int64_t k, int group, const uint8_t* codes, const S* scales) {
+        wgf_q4_weight* out = nullptr;
+        check(wgf_q4_weight_from_host(dev.raw(), n, k, (uint32_t)group, codes, DataType<S>::code, scales, &out));
+        return Q4Weight(out);
+    }
+    Q4Weight(const Q4Weight& o) : h_(o.h_) { check(wgf_q4_weight_retain(h_)); }
+    Q4Weight(Q4Weight&& o) noexcept : h_(o.h_) { o.h_ = nullptr; }
+    Q4Weight& operator=(Q4Weight o) noexcept {
+        std::swap(h_, o.h_);
+        return *this;
+    }
+    ~Q4Weight() {
+        if (h_) wgf_q4_weight_release(h_);
+    }
+    int64_t rows() const { return extents()[0]; }
+    int64_t columns() const { return extents()[1]; }
+    template <typename D> Tensor<2, D> dequantize() const {
+        wgf_tensor* out = nullptr;
+        check(wgf_q4_weight_dequantize(h_, DataType<D>::code, &out));
+        return Tensor<2, D>(out);
+    }
+    wgf_q4_weight* raw() const { return h_; }
+
+   private:
+    std::array<int64_t, 2> extents() const {
+        std::array<int64_t, 2> e{};
+        check(wgf_q4_weight_info(h_, &e[0], &e[1], nullptr, nullptr));
+        return e;
+    }
+    wgf_q4_weight* h_ = nullptr;
+};
+
+// 8-bit key/value cache (wgf_kv_cache_*); copies are handles on the same cache.  Calls run at once, in the order in
+// which they are made.  `counts`: how many of the call's tokens each sequence has (empty: all of them).
+template <typename D>
+class KvCache {
+   public:
+    KvCache(const Device& dev, int64_t batch, int64_t kv_heads, int64_t head_dim, int64_t capacity) : batch_(batch) {
+        check(wgf_kv_cache_create(dev.raw(), DataType<D>::code, batch, kv_heads, head_dim, capacity, &h_));
+    }
+    KvCache(const KvCache& o) : h_(o.h_), batch_(o.batch_) { check(wgf_kv_cache_retain(h_)); }
+    KvCache& operator=(KvCache o) noexcept {
+        std::swap(h_, o.h_);
+        std::swap(batch_, o.batch_);
+        return *this;
+    }
+    ~KvCache() {
+        if (h_) wgf_kv_cache_release(h_);
+    }
+    std::vector<int64_t> lengths() const {
+        std::vector<int64_t> n((size_t)batch_);
+        check(wgf_kv_cache_lengths(h_, n.data()));
+        return n;
+    }
+    void truncate(const std::vector<int64_t>& lengths) const { check(wgf_kv_cache_truncate(h_, numbers(lengths))); }
+    void append(const Tensor<4, D>& k, const Tensor<4, D>& v, const std::vector<int64_t>& counts = {}) const {
+        check(wgf_kv_cache_append(h_, k.raw(), v.raw(), counts.empty() ? nullptr : numbers(counts)));
+    }
+    Tensor<4, D> append_qk(const Tensor<4, D>& q, const Tensor<4, D>& k, const Tensor<4, D>& v, const Tensor<1, D>& q_weight,
+                           const Tensor<1, D>& k_weight, const Tensor<2, D>& cos, const Tensor<2, D>& sin, float eps,
+                           const std::vector<int64_t>& counts = {}) const {
+        wgf_tensor* out = nullptr;
+        check(wgf_kv_cache_append_qk(h_, q.raw(), k.raw(), v.raw(), q_weight.raw(), k_weight.raw(), cos.raw(), sin.raw(), eps,
+                                     counts.empty() ? nullptr : numbers(counts), &out));
+        return Tensor<4, D>(out);
+    }
+    Tensor<4, D> attention(const Tensor<4, D>& q, float scale, const std::vector<int64_t>& counts = {}) const {
+        wgf_tensor* out = nullptr;
+        check(wgf_kv_cache_attention(h_, q.raw(), scale, counts.empty() ? nullptr : numbers(counts), &out));
+        return Tensor<4, D>(out);
+    }
+    std::pair<Tensor<4, D>, Tensor<4, D>> read() const {
+        wgf_tensor *k = nullptr, *v = nullptr;
+        check(wgf_kv_cache_read(h_, &k, &v));
+        return {Tensor<4, D>(k), Tensor<4, D>(v)};
+    }
+
+   private:
+    const int64_t* numbers(const std::vector<int64_t>& v) const {
+        if ((int64_t)v.size() != batch_) throw Error(WGF_ERR_SHAPE, "one number for each sequence");
+        return v.data();
+    }
+    wgf_kv_cache* h_ = nullptr;
+    int64_t batch_ = 0;
+};
+
 // TensorSlice, src/tensor.rs:669-855: host copy of a materialised tensor with index access.
 template <int R, typename D>
 class TensorSlice {
@@ -380,6 +474,18 @@ class Tensor {
         check(wgf_tensor_attention(h_, k.raw(), v.raw(), mask ? mask->raw() : nullptr, causal ? 1 : 0, scale, &out));
         return Tensor(out);
     }
+    // Each head of this tensor (queries) and of k, [batch, heads, seq, head_dim], normed and rotated: one kernel.
+    std::pair<Tensor, Tensor> qk_norm_rope(const Tensor& k, const Tensor<1, D>& q_weight, const Tensor<1, D>& k_weight, const Tensor<2, D>& cos,
+                                           const Tensor<2, D>& sin, float eps, int64_t start) const {
+        static_assert(R == 3 || R == 4, "qk_norm_rope takes [heads, sequence, head_dim] or [batch, heads, sequence, head_dim]");
+        wgf_tensor *q_out = nullptr, *k_out = nullptr;
+        check(wgf_tensor_qk_norm_rope(h_, k.raw(), q_weight.raw(), k_weight.raw(), cos.raw(), sin.raw(), eps, start, &q_out, &k_out));
+        return {Tensor(q_out), Tensor(k_out)};
+    }
+    // This tensor [.., k] times the transposed 4-bit weights: [.., n]
+    Tensor mat_mul_q4(const Q4Weight& w) const;
+    // This [n, k] tensor as 4-bit weights; group is 32, 64 or 128.
+    Q4Weight quantize_q4(int group) const;
     // Queues the kernels of this tensor's graph without downloading (LazyTensorData::materialize).
     void materialize() const { check(wgf_tensor_materialize(h_)); }
 
@@ -415,6 +521,18 @@ class Tensor {
     }
     wgf_tensor* h_ = nullptr;
 };
+
+template <int R, typename D> Tensor<R, D> Tensor<R, D>::mat_mul_q4(const Q4Weight& w) const {
+    wgf_tensor* out = nullptr;
+    check(wgf_tensor_matmul_q4(h_, w.raw(), &out));
+    return Tensor(out);
+}
+template <int R, typename D> Q4Weight Tensor<R, D>::quantize_q4(int group) const {
+    static_assert(R == 2, "4-bit weights are made from a [rows, columns] tensor");
+    wgf_q4_weight* out = nullptr;
+    check(wgf_q4_weight_quantize(h_, (uint32_t)group, &out));
+    return Q4Weight(out);
+}
 
 // One request for several tensors of any rank and type (wgf_tensor_materialize_many): a
 // whole-tensor reduction among them is computed inside the row kernel of another one.

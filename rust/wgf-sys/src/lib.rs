@@ -86,7 +86,7 @@ macro_rules! opaque {
         }
     )*};
 }
-opaque!(wgf_device, wgf_buffer, wgf_tensor, wgf_comm, wgf_timing, wgf_schedule);
+opaque!(wgf_device, wgf_buffer, wgf_tensor, wgf_comm, wgf_timing, wgf_schedule, wgf_kv_cache, wgf_q4_weight);
 
 /// Layout {offset, shape, strides} + DataTypeEnum + buffer: src/layout.rs:33-38, src/tensor.rs:300-306.
 #[repr(C)]
@@ -413,6 +413,26 @@ extern "C" {
         eps: f32,
         out: *mut *mut wgf_tensor,
     ) -> i32;
+    /// Norm and rotation of queries and keys, lazily, as ONE kernel (no counterpart in the crate):
+    ///   y = x / sqrt(mean(x^2) + eps) * weight over each head's head_dim values, then
+    ///   out[d] = y[d] cos[p][d] - y[d + D/2] sin[p][d], out[d + D/2] = y[d + D/2] cos[p][d] + y[d] sin[p][d],
+    /// with p = start + the token's index.  q and k are [heads, seq, head_dim] or [batch, heads, seq, head_dim]
+    /// (any strides: a transposed view of a projection costs nothing) and may differ in their heads alone;
+    /// q_weight, k_weight [head_dim]; cos / sin [>= start + seq, head_dim / 2]; all of one element type.
+    /// head_dim is even and at most 512.  Everything is computed in f32 and rounded once (unlike
+    /// wgf_tensor_layer_norm and wgf_tensor_rope, which round after every step as the crate does).
+    pub fn wgf_tensor_qk_norm_rope(
+        q: *mut wgf_tensor,
+        k: *mut wgf_tensor,
+        q_weight: *mut wgf_tensor,
+        k_weight: *mut wgf_tensor,
+        cos: *mut wgf_tensor,
+        sin: *mut wgf_tensor,
+        eps: f32,
+        start: i64,
+        q_out: *mut *mut wgf_tensor,
+        k_out: *mut *mut wgf_tensor,
+    ) -> i32;
     /// LazyTensorData::materialize, src/tensor.rs:286-288: resolves the graph below `t`
     /// (src/compute_graph/resolve.rs:16-248) and queues its kernels; does not wait.
     pub fn wgf_tensor_materialize(t: *mut wgf_tensor) -> i32;
@@ -445,6 +465,100 @@ extern "C" {
     pub fn wgf_tensor_graphviz(t: *mut wgf_tensor, dst: *mut c_char, capacity: u64, needed: *mut u64) -> i32;
     /// Number of live graph nodes reachable from the graph `t` belongs to (debug aid).
     pub fn wgf_tensor_graph_size(t: *mut wgf_tensor, nodes: *mut u64) -> i32;
+    /// head_dim: a multiple of 8, at most 256.
+    pub fn wgf_kv_cache_create(
+        dev: *mut wgf_device,
+        dtype: u32,
+        batch: i64,
+        kv_heads: i64,
+        head_dim: i64,
+        capacity: i64,
+        out: *mut *mut wgf_kv_cache,
+    ) -> i32;
+    pub fn wgf_kv_cache_retain(cache: *mut wgf_kv_cache) -> i32;
+    pub fn wgf_kv_cache_release(cache: *mut wgf_kv_cache) -> i32;
+    /// Tokens of each sequence, `batch` numbers.
+    pub fn wgf_kv_cache_lengths(cache: *mut wgf_kv_cache, lengths: *mut i64) -> i32;
+    /// Takes tokens back (drafts that were not accepted) or empties sequences: `batch` new lengths, none
+    /// above the present one.  The tokens of the open block and of the one before it are still held in
+    /// the element type, so at least the last 64 can go; further back a length must be a multiple of 64
+    /// (WGF_ERR_UNSUPPORTED otherwise, and nothing is changed).
+    pub fn wgf_kv_cache_truncate(cache: *mut wgf_kv_cache, lengths: *const i64) -> i32;
+    /// k, v [batch, kv_heads, tokens, head_dim] behind each sequence's last token.  `counts` (NULL: all)
+    /// says how many of the tokens each sequence takes, from the first on; the rest is padding and not
+    /// read.  WGF_ERR_INVALID_ARGUMENT, and nothing is changed, if a sequence would not fit.
+    pub fn wgf_kv_cache_append(
+        cache: *mut wgf_kv_cache,
+        k: *mut wgf_tensor,
+        v: *mut wgf_tensor,
+        counts: *const i64,
+    ) -> i32;
+    /// wgf_tensor_qk_norm_rope and wgf_kv_cache_append in one launch, with every sequence's tokens at its own
+    /// positions (its length on): q [batch, heads, tokens, head_dim] comes back normed and rotated, k goes to
+    /// the cache.  cos / sin reach to the longest sequence's last new token.  Rows of q behind a sequence's
+    /// count come back as zeros.
+    pub fn wgf_kv_cache_append_qk(
+        cache: *mut wgf_kv_cache,
+        q: *mut wgf_tensor,
+        k: *mut wgf_tensor,
+        v: *mut wgf_tensor,
+        q_weight: *mut wgf_tensor,
+        k_weight: *mut wgf_tensor,
+        cos: *mut wgf_tensor,
+        sin: *mut wgf_tensor,
+        eps: f32,
+        counts: *const i64,
+        q_out: *mut *mut wgf_tensor,
+    ) -> i32;
+    /// softmax(scale * q K^T) V for q [batch, heads, tokens, head_dim], heads a multiple of kv_heads (query
+    /// head h reads kv head h * kv_heads / heads).  The queries stand at the last positions of their sequence
+    /// (with `counts`, the first counts[b] of them do and the others are padding) and each sees the tokens up
+    /// to its own.  A query before the sequence's first token, and a padding one, gives zeros.  Made for a
+    /// few tokens a sequence; scores, sums and products are f32 for every element type.
+    pub fn wgf_kv_cache_attention(
+        cache: *mut wgf_kv_cache,
+        q: *mut wgf_tensor,
+        scale: f32,
+        counts: *const i64,
+        out: *mut *mut wgf_tensor,
+    ) -> i32;
+    /// The values that the codes stand for: two tensors [batch, kv_heads, longest length, head_dim], zero
+    /// behind each sequence's end.
+    pub fn wgf_kv_cache_read(
+        cache: *mut wgf_kv_cache,
+        k: *mut *mut wgf_tensor,
+        v: *mut *mut wgf_tensor,
+    ) -> i32;
+    /// From a [n, k] tensor: scale = max|w| * (1/7) as a product in f32, rounded to the tensor's type; code =
+    /// w / scale rounded to the nearest (ties to even) + 8.  A group with a value that is not finite gets a NaN scale.
+    pub fn wgf_q4_weight_quantize(w: *mut wgf_tensor, group: u32, out: *mut *mut wgf_q4_weight) -> i32;
+    /// From codes that exist: `codes` [n][(k + 1) / 2] bytes, the even column in the low half; `scales`
+    /// [n][(k + group - 1) / group] of `scale_dtype`.
+    pub fn wgf_q4_weight_from_host(
+        dev: *mut wgf_device,
+        n: i64,
+        k: i64,
+        group: u32,
+        codes: *const u8,
+        scale_dtype: u32,
+        scales: *const c_void,
+        out: *mut *mut wgf_q4_weight,
+    ) -> i32;
+    pub fn wgf_q4_weight_retain(w: *mut wgf_q4_weight) -> i32;
+    pub fn wgf_q4_weight_release(w: *mut wgf_q4_weight) -> i32;
+    pub fn wgf_q4_weight_info(
+        w: *mut wgf_q4_weight,
+        n: *mut i64,
+        k: *mut i64,
+        group: *mut u32,
+        scale_dtype: *mut u32,
+    ) -> i32;
+    /// The values as a [n, k] tensor of `dtype`.
+    pub fn wgf_q4_weight_dequantize(w: *mut wgf_q4_weight, dtype: u32, out: *mut *mut wgf_tensor) -> i32;
+    /// x [.., k] times the transposed weights: [.., n] of x's type, lazily.  A few rows are one kernel that
+    /// reads the codes, with f32 sums of exact products; for many rows the weights are first written
+    /// out in x's type (their values rounded to it) and the matrix product runs on them.
+    pub fn wgf_tensor_matmul_q4(x: *mut wgf_tensor, w: *mut wgf_q4_weight, out: *mut *mut wgf_tensor) -> i32;
     /// Contiguous block partition of `n_units` over `world` ranks: the first n_units % world
     /// ranks get one extra unit.
     pub fn wgf_shard_range(n_units: i64, world: i32, rank: i32, begin: *mut i64, end: *mut i64) -> i32;

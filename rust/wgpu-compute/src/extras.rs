@@ -196,3 +196,231 @@ impl<const R: usize, D: DataType> Tensor<R, D> {
         check(status)
     }
 }
+
+// ---- decoding token by token ----------------------------------------------------------------------
+
+impl<D: DataType> Tensor<4, D> {
+    /// Each head of `self` (queries) and `k`, both [batch, heads, seq, head_dim], normed, scaled by its
+    /// weight and rotated by its position, `start` on: one kernel for both.
+    #[allow(clippy::too_many_arguments)]
+    pub fn qk_norm_rope(
+        &self,
+        k: &Self,
+        q_weight: &Tensor<1, D>,
+        k_weight: &Tensor<1, D>,
+        cos: &Tensor<2, D>,
+        sin: &Tensor<2, D>,
+        eps: f32,
+        start: usize,
+    ) -> (Self, Self) {
+        let (mut q_out, mut k_out) = (ptr::null_mut(), ptr::null_mut());
+        expect(unsafe {
+            sys::wgf_tensor_qk_norm_rope(
+                self.raw,
+                k.raw,
+                q_weight.raw,
+                k_weight.raw,
+                cos.raw,
+                sin.raw,
+                eps,
+                start as i64,
+                &mut q_out,
+                &mut k_out,
+            )
+        });
+        (Tensor::from_raw(q_out, &self.device), Tensor::from_raw(k_out, &self.device))
+    }
+}
+
+/// 8-bit key/value cache for `batch` sequences (`wgf_kv_cache_*`).  Its calls run at once, in the order
+/// in which they are made.
+pub struct KvCache<D> {
+    raw: *mut sys::wgf_kv_cache,
+    device: Device,
+    batch: usize,
+    datatype: std::marker::PhantomData<D>,
+}
+
+impl<D: DataType> KvCache<D> {
+    pub fn new(device: &Device, batch: usize, kv_heads: usize, head_dim: usize, capacity: usize) -> Result<Self, Error> {
+        let mut raw = ptr::null_mut();
+        check(unsafe {
+            sys::wgf_kv_cache_create(
+                device.raw,
+                D::WGSL_TYPE.code(),
+                batch as i64,
+                kv_heads as i64,
+                head_dim as i64,
+                capacity as i64,
+                &mut raw,
+            )
+        })?;
+        Ok(KvCache { raw, device: device.clone(), batch, datatype: std::marker::PhantomData })
+    }
+
+    fn numbers(&self, values: &[usize]) -> Vec<i64> {
+        assert_eq!(values.len(), self.batch, "one number for each sequence");
+        values.iter().map(|&v| v as i64).collect()
+    }
+
+    pub fn lengths(&self) -> Vec<usize> {
+        let mut out = vec![0i64; self.batch];
+        expect(unsafe { sys::wgf_kv_cache_lengths(self.raw, out.as_mut_ptr()) });
+        out.into_iter().map(|v| v as usize).collect()
+    }
+
+    /// Takes tokens back: new lengths, none above the present ones.
+    pub fn truncate(&self, lengths: &[usize]) -> Result<(), Error> {
+        check(unsafe { sys::wgf_kv_cache_truncate(self.raw, self.numbers(lengths).as_ptr()) })
+    }
+
+    /// k, v [batch, kv_heads, tokens, head_dim]; `counts`: tokens that each sequence takes (`None`: all).
+    pub fn append(&self, k: &Tensor<4, D>, v: &Tensor<4, D>, counts: Option<&[usize]>) -> Result<(), Error> {
+        let counts = counts.map(|c| self.numbers(c));
+        let counts = counts.as_ref().map_or(ptr::null(), |c| c.as_ptr());
+        check(unsafe { sys::wgf_kv_cache_append(self.raw, k.raw, v.raw, counts) })
+    }
+
+    /// Norm and rotation of q and k at each sequence's own positions, and append, in one launch; returns q.
+    #[allow(clippy::too_many_arguments)]
+    pub fn append_qk(
+        &self,
+        q: &Tensor<4, D>,
+        k: &Tensor<4, D>,
+        v: &Tensor<4, D>,
+        q_weight: &Tensor<1, D>,
+        k_weight: &Tensor<1, D>,
+        cos: &Tensor<2, D>,
+        sin: &Tensor<2, D>,
+        eps: f32,
+        counts: Option<&[usize]>,
+    ) -> Result<Tensor<4, D>, Error> {
+        let counts = counts.map(|c| self.numbers(c));
+        let counts = counts.as_ref().map_or(ptr::null(), |c| c.as_ptr());
+        let mut out = ptr::null_mut();
+        check(unsafe {
+            sys::wgf_kv_cache_append_qk(
+                self.raw,
+                q.raw,
+                k.raw,
+                v.raw,
+                q_weight.raw,
+                k_weight.raw,
+                cos.raw,
+                sin.raw,
+                eps,
+                counts,
+                &mut out,
+            )
+        })?;
+        Ok(Tensor::from_raw(out, &self.device))
+    }
+
+    /// softmax(scale * q K^T) V for q [batch, heads, tokens, head_dim] at the sequences' last positions.
+    pub fn attention(&self, q: &Tensor<4, D>, scale: f32, counts: Option<&[usize]>) -> Result<Tensor<4, D>, Error> {
+        let counts = counts.map(|c| self.numbers(c));
+        let counts = counts.as_ref().map_or(ptr::null(), |c| c.as_ptr());
+        let mut out = ptr::null_mut();
+        check(unsafe { sys::wgf_kv_cache_attention(self.raw, q.raw, scale, counts, &mut out) })?;
+        Ok(Tensor::from_raw(out, &self.device))
+    }
+
+    /// The values that the codes stand for: (k, v), each [batch, kv_heads, longest length, head_dim].
+    pub fn read(&self) -> Result<(Tensor<4, D>, Tensor<4, D>), Error> {
+        let (mut k, mut v) = (ptr::null_mut(), ptr::null_mut());
+        check(unsafe { sys::wgf_kv_cache_read(self.raw, &mut k, &mut v) })?;
+        Ok((Tensor::from_raw(k, &self.device), Tensor::from_raw(v, &self.device)))
+    }
+}
+
+impl<D> Clone for KvCache<D> {
+    /// A second handle on the same cache.
+    fn clone(&self) -> Self {
+        expect(unsafe { sys::wgf_kv_cache_retain(self.raw) });
+        KvCache { raw: self.raw, device: self.device.clone(), batch: self.batch, datatype: std::marker::PhantomData }
+    }
+}
+
+impl<D> Drop for KvCache<D> {
+    fn drop(&mut self) {
+        unsafe { sys::wgf_kv_cache_release(self.raw) };
+    }
+}
+
+/// 4-bit weights [n, k] with group scales (`wgf_q4_weight_*`).
+pub struct Q4Weight {
+    raw: *mut sys::wgf_q4_weight,
+    device: Device,
+}
+
+impl Q4Weight {
+    /// From codes that exist: [n][(k + 1) / 2] bytes, the even column in the low half, and scales [n][groups].
+    pub fn from_codes<S: DataType>(
+        device: &Device,
+        n: usize,
+        k: usize,
+        group: usize,
+        codes: &[u8],
+        scales: &[S],
+    ) -> Result<Self, Error> {
+        assert_eq!(codes.len(), n * ((k + 1) / 2), "two codes a byte, rows of whole bytes");
+        assert_eq!(scales.len(), n * ((k + group - 1) / group), "one scale for each row and group");
+        let mut raw = ptr::null_mut();
+        check(unsafe {
+            sys::wgf_q4_weight_from_host(
+                device.raw,
+                n as i64,
+                k as i64,
+                group as u32,
+                codes.as_ptr(),
+                S::WGSL_TYPE.code(),
+                scales.as_ptr() as *const core::ffi::c_void,
+                &mut raw,
+            )
+        })?;
+        Ok(Q4Weight { raw, device: device.clone() })
+    }
+
+    /// (n, k, group)
+    pub fn extents(&self) -> (usize, usize, usize) {
+        let (mut n, mut k, mut group) = (0i64, 0i64, 0u32);
+        expect(unsafe { sys::wgf_q4_weight_info(self.raw, &mut n, &mut k, &mut group, ptr::null_mut()) });
+        (n as usize, k as usize, group as usize)
+    }
+
+    pub fn dequantize<D: DataType>(&self) -> Result<Tensor<2, D>, Error> {
+        let mut out = ptr::null_mut();
+        check(unsafe { sys::wgf_q4_weight_dequantize(self.raw, D::WGSL_TYPE.code(), &mut out) })?;
+        Ok(Tensor::from_raw(out, &self.device))
+    }
+}
+
+impl Clone for Q4Weight {
+    /// A second handle on the same weights.
+    fn clone(&self) -> Self {
+        expect(unsafe { sys::wgf_q4_weight_retain(self.raw) });
+        Q4Weight { raw: self.raw, device: self.device.clone() }
+    }
+}
+
+impl Drop for Q4Weight {
+    fn drop(&mut self) {
+        unsafe { sys::wgf_q4_weight_release(self.raw) };
+    }
+}
+
+impl<D: DataType> Tensor<2, D> {
+    /// This [n, k] tensor as 4-bit weights; `group` is 32, 64 or 128.
+    pub fn quantize_q4(&self, group: usize) -> Result<Q4Weight, Error> {
+        let mut raw = ptr::null_mut();
+        check(unsafe { sys::wgf_q4_weight_quantize(self.raw, group as u32, &mut raw) })?;
+        Ok(Q4Weight { raw, device: self.device.clone() })
+    }
+}
+
+impl<const R: usize, D: DataType> Tensor<R, D> {
+    /// self [.., k] times the transposed 4-bit weights: [.., n].
+    pub fn mat_mul_q4(&self, w: &Q4Weight) -> Self {
+        self.build(|out| unsafe { sys::wgf_tensor_matmul_q4(self.raw, w.raw, out) })
+    }
+}

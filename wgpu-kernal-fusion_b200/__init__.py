@@ -131,6 +131,26 @@ class Device:
         (wgf_schedule_begin / _end); afterwards `s.launch()` replays them with one call."""
         return Schedule(self)
 
+    def kv_cache(self, batch, kv_heads, head_dim, capacity, dtype=F16):
+        """8-bit key/value cache for `batch` sequences of up to `capacity` tokens (wgf_kv_cache_*)."""
+        return KvCache(self, batch, kv_heads, head_dim, capacity, dtype)
+
+    def q4_weight(self, codes, scales, k, group, dtype=None):
+        """4-bit weights [n, k] from codes [n, (k + 1) // 2] (two columns a byte, the even one low) and scales
+        [n, groups] (dtype as for `tensor`)."""
+        codes = np.ascontiguousarray(codes, dtype=np.uint8)
+        if dtype is None:
+            dtype = F16 if np.asarray(scales).dtype == np.float16 else F32
+        scales = np.ascontiguousarray(scales, dtype=_NP[dtype])
+        n = codes.shape[0]
+        if group > 0 and (codes.shape != (n, (k + 1) // 2) or scales.shape != (n, -(-k // group))):
+            raise ValueError(f"codes {codes.shape} and scales {scales.shape} are not those of [{n}, {k}] in groups of {group}")
+        out = C.c_void_p()
+        check(lib().wgf_q4_weight_from_host(self.h, C.c_int64(n), C.c_int64(k), C.c_uint32(group),
+                                            codes.ctypes.data_as(C.c_void_p), C.c_uint32(dtype),
+                                            scales.ctypes.data_as(C.c_void_p), C.byref(out)))
+        return Q4Weight(self, out)
+
     def arange(self, start, end, step=1.0, dtype=F32):
         out = C.c_void_p()
         check(lib().wgf_tensor_arange(self.h, C.c_uint32(dtype), C.c_float(start), C.c_float(end),
@@ -345,6 +365,24 @@ class Tensor:
                                          C.c_float(scale), C.byref(out)))
         return Tensor(self.dev, out)
 
+    def qk_norm_rope(self, k, q_weight, k_weight, cos, sin, eps=1e-6, start=0):
+        """Each head of self (queries) and k normed, scaled by its weight and rotated by its position, start on:
+        one kernel for both (wgf_tensor_qk_norm_rope).  Returns (q, k)."""
+        q_out, k_out = C.c_void_p(), C.c_void_p()
+        check(lib().wgf_tensor_qk_norm_rope(self.h, k.h, q_weight.h, k_weight.h, cos.h, sin.h, C.c_float(eps), C.c_int64(start),
+                                            C.byref(q_out), C.byref(k_out)))
+        return Tensor(self.dev, q_out), Tensor(self.dev, k_out)
+
+    def quantize_q4(self, group=128):
+        """This [n, k] tensor as 4-bit weights (wgf_q4_weight_quantize)."""
+        out = C.c_void_p()
+        check(lib().wgf_q4_weight_quantize(self.h, C.c_uint32(group), C.byref(out)))
+        return Q4Weight(self.dev, out)
+
+    def mat_mul_q4(self, w):
+        """self [.., k] times the transposed 4-bit weights: [.., n] (wgf_tensor_matmul_q4)."""
+        return self._un(lambda h, out: lib().wgf_tensor_matmul_q4(h, w.h, out))
+
     def all_reduce(self, comm, op=OP_SUM):
         out = C.c_void_p()
         check(lib().wgf_tensor_all_reduce(self.h, comm.h, C.c_uint32(op), C.byref(out)))
@@ -489,6 +527,88 @@ class Schedule:
         if getattr(self, "h", None) and _lib is not None:
             _lib.wgf_schedule_destroy(self.h)
             self.h = None
+
+
+class KvCache:
+    """8-bit key/value cache (wgf_kv_cache_*).  Calls run at once, in the order in which they are made."""
+
+    def __init__(self, dev, batch, kv_heads, head_dim, capacity, dtype=F16):
+        self.dev, self.batch = dev, batch
+        self.h = C.c_void_p()
+        check(lib().wgf_kv_cache_create(dev.h, C.c_uint32(dtype), C.c_int64(batch), C.c_int64(kv_heads), C.c_int64(head_dim),
+                                        C.c_int64(capacity), C.byref(self.h)))
+
+    def __del__(self):
+        if getattr(self, "h", None) and _lib is not None:
+            _lib.wgf_kv_cache_release(self.h)
+            self.h = None
+
+    def _numbers(self, values):
+        if values is None:
+            return None
+        if len(values) != self.batch:
+            raise ValueError(f"{len(values)} numbers for {self.batch} sequences")
+        return _i64(values)
+
+    @property
+    def lengths(self):
+        out = (C.c_int64 * self.batch)()
+        check(lib().wgf_kv_cache_lengths(self.h, out))
+        return list(out)
+
+    def truncate(self, lengths):
+        """Takes tokens back: new lengths, none above the present ones (wgf_kv_cache_truncate)."""
+        check(lib().wgf_kv_cache_truncate(self.h, self._numbers(lengths)))
+
+    def append(self, k, v, counts=None):
+        """k, v [batch, kv_heads, tokens, head_dim]; counts: tokens that each sequence takes (default: all)."""
+        check(lib().wgf_kv_cache_append(self.h, k.h, v.h, self._numbers(counts)))
+
+    def append_qk(self, q, k, v, q_weight, k_weight, cos, sin, eps=1e-6, counts=None):
+        """Norm and rotation of q and k at each sequence's own positions, and append, in one launch; returns q."""
+        out = C.c_void_p()
+        check(lib().wgf_kv_cache_append_qk(self.h, q.h, k.h, v.h, q_weight.h, k_weight.h, cos.h, sin.h, C.c_float(eps),
+                                           self._numbers(counts), C.byref(out)))
+        return Tensor(self.dev, out)
+
+    def attention(self, q, scale=None, counts=None):
+        """softmax(scale q K^T) V for q [batch, heads, tokens, head_dim] at the sequences' last positions."""
+        if scale is None:
+            scale = 1.0 / float(np.sqrt(q.shape[-1]))
+        out = C.c_void_p()
+        check(lib().wgf_kv_cache_attention(self.h, q.h, C.c_float(scale), self._numbers(counts), C.byref(out)))
+        return Tensor(self.dev, out)
+
+    def read(self):
+        """(k, v): the values that the codes stand for, [batch, kv_heads, longest length, head_dim]."""
+        k, v = C.c_void_p(), C.c_void_p()
+        check(lib().wgf_kv_cache_read(self.h, C.byref(k), C.byref(v)))
+        return Tensor(self.dev, k), Tensor(self.dev, v)
+
+
+class Q4Weight:
+    """4-bit weights with group scales (wgf_q4_weight_*): Tensor.quantize_q4, Device.q4_weight."""
+
+    def __init__(self, dev, handle):
+        self.dev = dev
+        self.h = handle
+
+    def __del__(self):
+        if getattr(self, "h", None) and _lib is not None:
+            _lib.wgf_q4_weight_release(self.h)
+            self.h = None
+
+    @property
+    def info(self):
+        """(n, k, group, scale dtype)"""
+        n, k, g, d = C.c_int64(), C.c_int64(), C.c_uint32(), C.c_uint32()
+        check(lib().wgf_q4_weight_info(self.h, C.byref(n), C.byref(k), C.byref(g), C.byref(d)))
+        return n.value, k.value, g.value, d.value
+
+    def dequantize(self, dtype=F32):
+        out = C.c_void_p()
+        check(lib().wgf_q4_weight_dequantize(self.h, C.c_uint32(dtype), C.byref(out)))
+        return Tensor(self.dev, out)
 
 
 def shard_range(n_units, world, rank):

@@ -4,6 +4,7 @@
 #include <mutex>
 
 #include "comm.hpp"
+#include "decode.hpp"
 #include "graph.hpp"
 #include "half.hpp"
 
@@ -22,6 +23,14 @@ struct wgf_tensor {
 };
 struct wgf_comm {
     std::shared_ptr<Comm> ref;
+};
+struct wgf_kv_cache {
+    KvCacheRef ref;
+    std::atomic<int> rc{1};
+};
+struct wgf_q4_weight {
+    Q4Ref ref;
+    std::atomic<int> rc{1};
 };
 // Event pairs of the kernels (or the copy) one call queued; read with wgf_timing_elapsed_ns.
 struct wgf_timing {
@@ -151,6 +160,34 @@ void timed(const DeviceRef& devref, wgf_timing** timing, F&& f) {
     dev.sink = nullptr;
     dev.timing = was;
     if (timing) *timing = t.release();
+}
+
+// Operands of a call that runs at once: resolved now (their own kernels are timed in their graphs), and held by a recording.
+TensorData operand(const DeviceRef& dev, wgf_tensor* t) {
+    WGF_CHECK(t->node->dev == dev, WGF_ERR_INVALID_ARGUMENT, "operands live on different devices");
+    TensorData d = resolve(t->node);
+    dev->note_recorded_buffer(d.buf);
+    return d;
+}
+// Runs `f`; with the device's timing on, its kernels' times belong to the graph of the tensor that `f` returns.
+template <typename F> wgf_tensor* run_now(const DeviceRef& dev, F&& f) {
+    std::vector<TimingRecord> recs;
+    dev->sink = dev->timing ? &recs : nullptr;
+    TensorData out;
+    try {
+        out = f();
+    } catch (...) {
+        dev->sink = nullptr;
+        for (auto& r : recs) {
+            dev->recycle(r.start);
+            dev->recycle(r.stop);
+        }
+        throw;
+    }
+    dev->sink = nullptr;
+    NodeRef n = make_tensor(dev, out);
+    graph_of(n)->timings = std::move(recs);
+    return wrap(n);
 }
 
 }  // namespace
@@ -932,6 +969,179 @@ int32_t wgf_tensor_graph_size(wgf_tensor* t, uint64_t* nodes) {
         REQUIRE(t);
         REQUIRE(nodes);
         *nodes = graph_of(t->node)->live_nodes;
+    })
+}
+
+// ---------------------------------------------------------------- decode path
+int32_t wgf_tensor_qk_norm_rope(wgf_tensor* q, wgf_tensor* k, wgf_tensor* q_weight, wgf_tensor* k_weight, wgf_tensor* cos,
+                                wgf_tensor* sin, float eps, int64_t start, wgf_tensor** q_out, wgf_tensor** k_out) {
+    GRAPH_GUARD({
+        REQUIRE(q);
+        REQUIRE(k);
+        REQUIRE(q_weight);
+        REQUIRE(k_weight);
+        REQUIRE(cos);
+        REQUIRE(sin);
+        REQUIRE(q_out);
+        REQUIRE(k_out);
+        auto both = op_qk_norm_rope(q->node, k->node, q_weight->node, k_weight->node, cos->node, sin->node, eps, start);
+        *q_out = wrap(both.first);
+        *k_out = wrap(both.second);
+    })
+}
+
+int32_t wgf_kv_cache_create(wgf_device* dev, uint32_t dtype, int64_t batch, int64_t kv_heads, int64_t head_dim, int64_t capacity,
+                            wgf_kv_cache** out) {
+    GRAPH_GUARD({
+        REQUIRE(dev);
+        REQUIRE(out);
+        *out = nullptr;
+        WGF_CHECK(valid_dtype(dtype), WGF_ERR_DTYPE, "unknown element type");
+        *out = new wgf_kv_cache{kv_cache_create(dev->ref, (DType)dtype, batch, kv_heads, head_dim, capacity)};
+    })
+}
+int32_t wgf_kv_cache_retain(wgf_kv_cache* cache) {
+    return guard([&] {
+        REQUIRE(cache);
+        cache->rc++;
+    });
+}
+int32_t wgf_kv_cache_release(wgf_kv_cache* cache) {
+    GRAPH_GUARD({
+        REQUIRE(cache);
+        if (--cache->rc == 0) delete cache;
+    })
+}
+int32_t wgf_kv_cache_lengths(wgf_kv_cache* cache, int64_t* lengths) {
+    GRAPH_GUARD({
+        REQUIRE(cache);
+        REQUIRE(lengths);
+        std::copy(cache->ref->lengths.begin(), cache->ref->lengths.end(), lengths);
+    })
+}
+int32_t wgf_kv_cache_truncate(wgf_kv_cache* cache, const int64_t* lengths) {
+    GRAPH_GUARD({
+        REQUIRE(cache);
+        REQUIRE(lengths);
+        kv_cache_truncate(*cache->ref, lengths);
+    })
+}
+int32_t wgf_kv_cache_append(wgf_kv_cache* cache, wgf_tensor* k, wgf_tensor* v, const int64_t* counts) {
+    GRAPH_GUARD({
+        REQUIRE(cache);
+        REQUIRE(k);
+        REQUIRE(v);
+        const DeviceRef& dev = cache->ref->dev;
+        TensorData kd = operand(dev, k);
+        TensorData vd = operand(dev, v);
+        kv_cache_append(*cache->ref, kd, vd, counts);
+    })
+}
+int32_t wgf_kv_cache_append_qk(wgf_kv_cache* cache, wgf_tensor* q, wgf_tensor* k, wgf_tensor* v, wgf_tensor* q_weight,
+                               wgf_tensor* k_weight, wgf_tensor* cos, wgf_tensor* sin, float eps, const int64_t* counts,
+                               wgf_tensor** q_out) {
+    GRAPH_GUARD({
+        REQUIRE(cache);
+        REQUIRE(q);
+        REQUIRE(k);
+        REQUIRE(v);
+        REQUIRE(q_weight);
+        REQUIRE(k_weight);
+        REQUIRE(cos);
+        REQUIRE(sin);
+        REQUIRE(q_out);
+        const DeviceRef& dev = cache->ref->dev;
+        wgf_tensor* in[7] = {q, k, v, q_weight, k_weight, cos, sin};
+        TensorData d[7];
+        for (int i = 0; i < 7; ++i) d[i] = operand(dev, in[i]);
+        *q_out = run_now(dev, [&] { return kv_cache_append_qk(*cache->ref, d[0], d[1], d[2], d[3], d[4], d[5], d[6], eps, counts); });
+    })
+}
+int32_t wgf_kv_cache_attention(wgf_kv_cache* cache, wgf_tensor* q, float scale, const int64_t* counts, wgf_tensor** out) {
+    GRAPH_GUARD({
+        REQUIRE(cache);
+        REQUIRE(q);
+        REQUIRE(out);
+        const DeviceRef& dev = cache->ref->dev;
+        TensorData qd = operand(dev, q);
+        *out = run_now(dev, [&] { return kv_cache_attention(*cache->ref, qd, scale, counts); });
+    })
+}
+int32_t wgf_kv_cache_read(wgf_kv_cache* cache, wgf_tensor** k, wgf_tensor** v) {
+    GRAPH_GUARD({
+        REQUIRE(cache);
+        REQUIRE(k);
+        REQUIRE(v);
+        const DeviceRef& dev = cache->ref->dev;
+        TensorData kd, vd;
+        wgf_tensor* first = run_now(dev, [&] {
+            kv_cache_read(*cache->ref, kd, vd);
+            return kd;
+        });
+        *k = first;
+        *v = wrap(make_tensor(dev, vd));
+    })
+}
+
+int32_t wgf_q4_weight_quantize(wgf_tensor* w, uint32_t group, wgf_q4_weight** out) {
+    GRAPH_GUARD({
+        REQUIRE(w);
+        REQUIRE(out);
+        *out = nullptr;
+        const DeviceRef dev = w->node->dev;
+        dev->refuse_while_recording("making 4-bit weights");
+        TensorData d = operand(dev, w);
+        *out = new wgf_q4_weight{q4_quantize(dev, d, group)};
+    })
+}
+int32_t wgf_q4_weight_from_host(wgf_device* dev, int64_t n, int64_t k, uint32_t group, const uint8_t* codes, uint32_t scale_dtype,
+                                const void* scales, wgf_q4_weight** out) {
+    GRAPH_GUARD({
+        REQUIRE(dev);
+        REQUIRE(codes);
+        REQUIRE(scales);
+        REQUIRE(out);
+        *out = nullptr;
+        WGF_CHECK(valid_dtype(scale_dtype), WGF_ERR_DTYPE, "unknown element type");
+        *out = new wgf_q4_weight{q4_from_host(dev->ref, n, k, group, codes, (DType)scale_dtype, scales)};
+    })
+}
+int32_t wgf_q4_weight_retain(wgf_q4_weight* w) {
+    return guard([&] {
+        REQUIRE(w);
+        w->rc++;
+    });
+}
+int32_t wgf_q4_weight_release(wgf_q4_weight* w) {
+    GRAPH_GUARD({
+        REQUIRE(w);
+        if (--w->rc == 0) delete w;
+    })
+}
+int32_t wgf_q4_weight_info(wgf_q4_weight* w, int64_t* n, int64_t* k, uint32_t* group, uint32_t* scale_dtype) {
+    return guard([&] {
+        REQUIRE(w);
+        if (n) *n = w->ref->n;
+        if (k) *k = w->ref->k;
+        if (group) *group = (uint32_t)w->ref->group;
+        if (scale_dtype) *scale_dtype = (uint32_t)w->ref->scale_dtype;
+    });
+}
+int32_t wgf_q4_weight_dequantize(wgf_q4_weight* w, uint32_t dtype, wgf_tensor** out) {
+    GRAPH_GUARD({
+        REQUIRE(w);
+        REQUIRE(out);
+        WGF_CHECK(valid_dtype(dtype), WGF_ERR_DTYPE, "unknown element type");
+        const DeviceRef dev = w->ref->dev;
+        *out = run_now(dev, [&] { return q4_dequantize(*dev, *w->ref, (DType)dtype); });
+    })
+}
+int32_t wgf_tensor_matmul_q4(wgf_tensor* x, wgf_q4_weight* w, wgf_tensor** out) {
+    GRAPH_GUARD({
+        REQUIRE(x);
+        REQUIRE(w);
+        REQUIRE(out);
+        *out = wrap(op_matmul_q4(x->node, w->ref));
     })
 }
 

@@ -1,0 +1,125 @@
+// Pieces that the kernels of the decode path share: conversions, wide loads, the norm and rotation
+// of one head, and the rounding of a value to its code.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cstdint>
+
+namespace wgf {
+namespace decode {
+
+template <typename T> __device__ __forceinline__ float to_f(T v);
+template <> __device__ __forceinline__ float to_f<float>(float v) { return v; }
+template <> __device__ __forceinline__ float to_f<__half>(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_f(float v);
+template <> __device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// VEC elements moved as one access
+template <typename T, int VEC> struct alignas(sizeof(T) * VEC) Pack {
+    T v[VEC];
+};
+
+// round-half-even(k * x / den) for an integer k <= 127 and den > 0, |k * x / den| <= 127 or so, as if
+// the quotient were exact: the codes do not depend on how a division rounds.  k * x is held in two
+// floats and the remainder of the nearest integer is exact by the fused multiply-add, so comparing it with
+// half a step tells which side of the border the value is on.
+__device__ __forceinline__ int exact_code(float x, float k, float den, float inv) {
+    const float p = __fmul_rn(k, x), pl = __fmaf_rn(k, x, -p);
+    float r = rintf(__fmul_rn(p, inv));
+    const float e = __fmaf_rn(-r, den, p);         // p - r * den, exact
+    const float h = 0.5f * den;
+    const float over = (e - h) + pl, under = (e + h) + pl;   // > 0: above the upper border; < 0: below the lower one
+    if (over > 0.f || (over == 0.f && (((int)r) & 1))) r += 1.f;
+    else if (under < 0.f || (under == 0.f && (((int)r) & 1))) r -= 1.f;
+    return (int)r;
+}
+
+// The largest |x| as an ordered integer: NaN above infinity above every number, so that a block that holds
+// either is told apart whatever the order of its values.
+__device__ __forceinline__ unsigned abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+// ---- one head: y = x / sqrt(mean(x^2) + eps) * w, then rotated by the position's angle -------------------
+// A group of `lanes` (a power of two, at most 32, neighbours in a warp) holds a row: lane l has the chunks
+// l, l + lanes, ... of VEC values of the first half, and the same chunks of the second half, which are the
+// partners of the rotation.  Everything is f32; the caller rounds once.
+template <typename T, int VEC, int NCH> struct HeadRow {
+    float lo[NCH][VEC], hi[NCH][VEC];
+
+    __device__ __forceinline__ void load(const T* row, int half, int lane, int lanes) {
+        typedef Pack<T, VEC> V;
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) {
+            const int j = (lane + c * lanes) * VEC;
+            if (j < half) {
+                const V a = *reinterpret_cast<const V*>(row + j), b = *reinterpret_cast<const V*>(row + half + j);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    lo[c][e] = to_f<T>(a.v[e]);
+                    hi[c][e] = to_f<T>(b.v[e]);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) lo[c][e] = hi[c][e] = 0.f;
+            }
+        }
+    }
+    // All 32 lanes of the warp take part.
+    __device__ __forceinline__ float inverse_rms(int half, int lanes, float eps) const {
+        float s = 0.f;
+#pragma unroll
+        for (int c = 0; c < NCH; ++c)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) s += lo[c][e] * lo[c][e] + hi[c][e] * hi[c][e];
+        for (int m = lanes >> 1; m >= 1; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
+        return 1.0f / sqrtf(s / (float)(2 * half) + eps);
+    }
+    __device__ __forceinline__ void norm_rotate(const HeadRow& w, const float (&cs)[NCH][VEC], const float (&sn)[NCH][VEC], float r) {
+#pragma unroll
+        for (int c = 0; c < NCH; ++c)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float a = lo[c][e] * r * w.lo[c][e], b = hi[c][e] * r * w.hi[c][e];
+                lo[c][e] = a * cs[c][e] - b * sn[c][e];
+                hi[c][e] = b * cs[c][e] + a * sn[c][e];
+            }
+    }
+    __device__ __forceinline__ void store(T* row, int half, int lane, int lanes) const {
+        typedef Pack<T, VEC> V;
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) {
+            const int j = (lane + c * lanes) * VEC;
+            if (j >= half) continue;
+            V a, b;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                a.v[e] = from_f<T>(lo[c][e]);
+                b.v[e] = from_f<T>(hi[c][e]);
+            }
+            *reinterpret_cast<V*>(row + j) = a;
+            *reinterpret_cast<V*>(row + half + j) = b;
+        }
+    }
+};
+template <typename T, int VEC, int NCH>
+__device__ __forceinline__ void load_half(const T* p, int half, int lane, int lanes, float (&v)[NCH][VEC]) {
+    typedef Pack<T, VEC> V;
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+        const int j = (lane + c * lanes) * VEC;
+        if (j < half) {
+            const V a = *reinterpret_cast<const V*>(p + j);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v[c][e] = to_f<T>(a.v[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v[c][e] = 0.f;
+        }
+    }
+}
+
+}  // namespace decode
+}  // namespace wgf

@@ -8,6 +8,7 @@
 
 #include "attention.hpp"
 #include "comm.hpp"
+#include "decode.hpp"
 #include "half.hpp"
 #include "matmul.hpp"
 
@@ -386,6 +387,37 @@ NodeRef op_rope(const NodeRef& x, const NodeRef& cos, const NodeRef& sin) {
     NodeRef x1 = op_narrow(x, 2, 0, d / 2), x2 = op_narrow(x, 2, d / 2, d - d / 2);
     NodeRef rot = op_cat({make_unary(x2, WGF_OP_NEG), x1}, 2);
     return make_binary(make_binary(x, c, WGF_OP_MUL), make_binary(rot, s, WGF_OP_MUL), WGF_OP_ADD);
+}
+
+std::pair<NodeRef, NodeRef> op_qk_norm_rope(const NodeRef& q, const NodeRef& k, const NodeRef& wq, const NodeRef& wk, const NodeRef& cos,
+                                            const NodeRef& sin, float eps, int64_t start) {
+    const int r = q->rank();
+    WGF_CHECK((r == 3 || r == 4) && k->rank() == r, WGF_ERR_RANK, "qk_norm_rope takes q and k as [heads, seq, dim] or [batch, heads, seq, dim]");
+    const int64_t S = q->shape[r - 2], D = q->shape[r - 1];
+    WGF_CHECK((r == 3 || q->shape[0] == k->shape[0]) && k->shape[r - 2] == S && k->shape[r - 1] == D, WGF_ERR_SHAPE,
+              "qk_norm_rope: q and k differ in more than their heads");
+    WGF_CHECK(D >= 2 && D % 2 == 0 && D <= kMaxNormDim, WGF_ERR_UNSUPPORTED, "qk_norm_rope needs an even head_dim up to 512");
+    WGF_CHECK(wq->rank() == 1 && wk->rank() == 1 && wq->shape[0] == D && wk->shape[0] == D, WGF_ERR_SHAPE, "qk_norm_rope weights must be [head_dim]");
+    WGF_CHECK(cos->rank() == 2 && sin->rank() == 2 && cos->shape == sin->shape && cos->shape[1] * 2 == D, WGF_ERR_SHAPE,
+              "qk_norm_rope cos / sin must be equal [positions, head_dim / 2]");
+    WGF_CHECK(start >= 0 && start <= cos->shape[0] && S <= cos->shape[0] - start, WGF_ERR_SHAPE, "qk_norm_rope: positions past the end of cos / sin");
+    for (const NodeRef& n : {k, wq, wk, cos, sin}) WGF_CHECK(n->dtype == q->dtype, WGF_ERR_DTYPE, "qk_norm_rope element types differ");
+    const int64_t nq = q->numel(), nk = k->numel(), at = qk_second_offset(nq);
+    auto both = new_node(NodeKind::QkNormRope, q->dev, {at + nk}, q->dtype, {q, k, wq, wk, cos, sin});
+    both->imm = eps;
+    both->starts = {start, at};
+    return {op_reshape(view_slice(both, {0}, {nq}), q->shape), op_reshape(view_slice(both, {at}, {at + nk}), k->shape)};
+}
+
+NodeRef op_matmul_q4(const NodeRef& x, const std::shared_ptr<Q4Weight>& w) {
+    WGF_CHECK(x->rank() >= 1, WGF_ERR_RANK, "the product with 4-bit weights needs rank >= 1");
+    WGF_CHECK(x->dev == w->dev, WGF_ERR_INVALID_ARGUMENT, "operands live on different devices");
+    WGF_CHECK(x->shape.back() == w->k, WGF_ERR_SHAPE, "the last axis differs from the weights' columns");
+    std::vector<int64_t> s = x->shape;
+    s.back() = w->n;
+    auto n = new_node(NodeKind::MatMulQ4, x->dev, s, x->dtype, {x});
+    n->q4 = w;
+    return n;
 }
 
 NodeRef op_attention(const NodeRef& q, const NodeRef& k, const NodeRef& v, const NodeRef& mask, bool causal, float scale) {
@@ -1166,6 +1198,17 @@ TensorData resolve_node(Node* n) {
             out = run_rope(dev, x, c, s);
             break;
         }
+        case NodeKind::QkNormRope: {
+            TensorData in[6];
+            for (int i = 0; i < 6; ++i) in[i] = resolve_node(n->inputs[i].get());
+            out = run_qk_norm_rope(dev, in[0], in[1], in[2], in[3], in[4], in[5], n->imm, n->starts[0], n->starts[1]);
+            break;
+        }
+        case NodeKind::MatMulQ4: {
+            TensorData x = resolve_node(n->inputs[0].get());
+            out = run_matmul_q4(dev, x, *n->q4);
+            break;
+        }
         case NodeKind::Attention: {
             TensorData q = resolve_node(n->inputs[0].get());
             TensorData k = resolve_node(n->inputs[1].get());
@@ -1333,7 +1376,7 @@ void resolve_many(const std::vector<NodeRef>& nodes) {
 // ---------------------------------------------------------------------------------------
 std::string graphviz(const NodeRef& root) {
     static const char* kinds[] = {"tensor", "element_wise", "pair_wise", "reduce", "mat_mul",
-                                  "map_layout", "resize", "slice_assign", "all_reduce", "attention", "rope"};
+                                  "map_layout", "resize", "slice_assign", "all_reduce", "attention", "rope", "qk_norm_rope", "mat_mul_q4"};
     std::ostringstream s;
     s << "digraph compute_graph {\n";
     std::unordered_set<Node*> seen;

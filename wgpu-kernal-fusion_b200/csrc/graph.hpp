@@ -15,11 +15,14 @@
 namespace wgf {
 
 struct Comm;
+struct Q4Weight;
 
 enum class NodeKind : uint8_t {
     Tensor, ElementWise, PairWise, Reduce, MatMul, MapLayout, Resize, SliceAssign, AllReduce,
     Attention,  // fused causal softmax attention (no counterpart in the crate); imm = scale
-    Rope        // rotary embedding as one kernel; inputs x, cos, sin
+    Rope,       // rotary embedding as one kernel; inputs x, cos, sin
+    QkNormRope, // norm and rotation of queries and keys; inputs q, k, their weights, cos, sin; imm = eps, starts[0] = first position
+    MatMulQ4    // product with 4-bit weights
 };
 
 struct ViewOp {
@@ -51,6 +54,7 @@ struct Node {
     ViewOp view;
     std::vector<int64_t> new_shape, fill_shape, starts, ends;
     std::shared_ptr<Comm> comm;
+    std::shared_ptr<Q4Weight> q4;
     // Scratch of the resolver, used instead of hash containers keyed by node: a "set" is an epoch
     // number, and the node belongs to it while the slot of that kind carries the epoch.
     struct Scratch {
@@ -117,6 +121,12 @@ NodeRef op_layer_norm(const NodeRef& x, const NodeRef& weight, float eps);
 NodeRef op_softmax(const NodeRef& x);
 NodeRef op_softmax_last_dim(const NodeRef& x);
 NodeRef op_rope(const NodeRef& x, const NodeRef& cos, const NodeRef& sin);
+// Every head of q and k [.., seq, dim] normed, scaled by its weight [dim] and rotated by rows start, start + 1, ... of
+// cos / sin [positions, dim / 2]: one kernel.
+std::pair<NodeRef, NodeRef> op_qk_norm_rope(const NodeRef& q, const NodeRef& k, const NodeRef& wq, const NodeRef& wk, const NodeRef& cos,
+                                            const NodeRef& sin, float eps, int64_t start);
+// x [.., k] times the transposed 4-bit weights [n, k].
+NodeRef op_matmul_q4(const NodeRef& x, const std::shared_ptr<Q4Weight>& w);
 // softmax(scale * q k^T + mask) v over [batch*heads, seq, head_dim] tensors.  `mask` is an
 // additive [seq, seq] tensor or null; with a null mask `causal` masks the keys after each
 // query and, where the shapes allow (16-bit, head_dim 128, seq a multiple of 128), one fused

@@ -680,6 +680,7 @@ void Device::begin_recording() {
     }
     arena_ = std::make_shared<Arena>();
     recorded_inputs_.clear();
+    recorded_steps_.clear();
     recording_from_ = launches.load();
 }
 
@@ -696,8 +697,12 @@ Device::Recorded Device::end_recording() {
     r.arena = arena_;
     r.kernels = launches.load() - recording_from_;
     r.inputs.swap(recorded_inputs_);
+    r.steps.swap(recorded_steps_);
     arena_.reset();
-    if (dry) return r;
+    if (dry) {
+        for (auto& s : r.steps) s->commit();
+        return r;
+    }
     make_current();
     cudaError_t e = cudaStreamEndCapture(stream, &r.graph);
     if (e == cudaSuccess) e = cudaGraphInstantiate(&r.exec, r.graph, 0);
@@ -707,15 +712,19 @@ Device::Recorded Device::end_recording() {
         destroy_recorded(r);
         fail(WGF_ERR_CUDA, std::string("recording the schedule failed: ") + cudaGetErrorString(e));
     }
+    for (auto& s : r.steps) s->commit();   // that was the first launch
     return r;
 }
 
 void Device::replay(const Recorded& r) {
     refuse_while_recording("replaying a schedule");
+    for (auto& s : r.steps) s->check();
     launches += r.kernels;
-    if (dry) return;
-    make_current();
-    WGF_CUDA(cudaGraphLaunch(r.exec, stream));
+    if (!dry) {
+        make_current();
+        WGF_CUDA(cudaGraphLaunch(r.exec, stream));
+    }
+    for (auto& s : r.steps) s->commit();
 }
 
 void Device::destroy_recorded(Recorded& r) {
@@ -729,6 +738,7 @@ void Device::destroy_recorded(Recorded& r) {
     r.exec = nullptr;
     r.graph = nullptr;
     r.inputs.clear();   // no replay can read them any more
+    r.steps.clear();
     if (r.arena) {
         std::multimap<size_t, void*> blocks;
         {

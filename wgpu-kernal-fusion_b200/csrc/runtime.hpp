@@ -69,6 +69,15 @@ struct TensorData {
     explicit operator bool() const { return (bool)buf; }
 };
 
+// Something on the host that moves on with every launch of a recorded schedule (a cache whose recorded
+// appends lengthen it).  `check` fails, before anything is queued, where a launch would not fit; `commit`
+// follows a launch.
+struct ReplayStep {
+    virtual ~ReplayStep() {}
+    virtual void check() const = 0;
+    virtual void commit() = 0;
+};
+
 struct TimingRecord {
     cudaEvent_t start = nullptr, stop = nullptr;
     const char* what = "";
@@ -159,6 +168,7 @@ struct Device : std::enable_shared_from_this<Device> {
         // reads their addresses again, so the schedule holds them until it is destroyed -- a
         // caller that drops its handle does not send the block back to the pool under the graph.
         std::vector<BufferRef> inputs;
+        std::vector<std::shared_ptr<ReplayStep>> steps;
     };
     bool recording() const { return (bool)arena_; }
     void begin_recording();
@@ -172,6 +182,8 @@ struct Device : std::enable_shared_from_this<Device> {
     // that do not belong to the recording's own arena (see Recorded::inputs).  No-op otherwise.
     void note_recorded_buffer(const BufferRef& b);
     const std::shared_ptr<Arena>& arena() const { return arena_; }
+    // The steps of the recording under way.
+    std::vector<std::shared_ptr<ReplayStep>>& recorded_steps() { return recorded_steps_; }
 
     // Timing sink: while set, every launch appends an event pair to it.
     std::vector<TimingRecord>* sink = nullptr;
@@ -201,6 +213,7 @@ struct Device : std::enable_shared_from_this<Device> {
     std::vector<Deferred> deferred_;
     std::shared_ptr<Arena> arena_;     // non-null while recording
     std::vector<BufferRef> recorded_inputs_;
+    std::vector<std::shared_ptr<ReplayStep>> recorded_steps_;
     uint64_t recording_from_ = 0;      // value of `launches` when recording began
     void drain_deferred_locked();
     void* raw_alloc(size_t block);
