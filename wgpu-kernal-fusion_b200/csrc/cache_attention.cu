@@ -77,12 +77,6 @@ __device__ __forceinline__ void mma(float (&c)[4], unsigned a0, unsigned a1, uns
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void copy16(void* dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
-}
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 // Shared memory of a CTA: the warps' rings, then the queries as A operands:
 // [dims / 64][half of the chunk's four steps][lane] { step: a0 hi, a1 lo, a2 hi, a3 lo } x 2, and per row the power of
 // two that its queries were scaled by.

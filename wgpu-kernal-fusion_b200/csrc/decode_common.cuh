@@ -23,6 +23,35 @@ template <typename T, int VEC> struct alignas(sizeof(T) * VEC) Pack {
     T v[VEC];
 };
 
+// Shared memory by its own 32-bit addresses
+__device__ __forceinline__ unsigned shared_address(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ uint4 shared_16(unsigned at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ float2 shared_float2(unsigned at) {
+    float2 v;
+    asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ unsigned shared_word(unsigned at) {
+    unsigned v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
+// From global to shared memory without waiting: 16, 8 or 4 bytes
+__device__ __forceinline__ void copy16_at(unsigned dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+template <int BYTES> __device__ __forceinline__ void copy_at(unsigned dst, const void* src) {
+    static_assert(BYTES == 4 || BYTES == 8, "");
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
+}
+__device__ __forceinline__ void copy16(void* dst, const void* src) { copy16_at(shared_address(dst), src); }
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
 // round-half-even(k * x / den) for an integer k <= 127 and den > 0, |k * x / den| <= 127 or so, as if
 // the quotient were exact: the codes do not depend on how a division rounds.  k * x is held in two
 // floats and the remainder of the nearest integer is exact by the fused multiply-add, so comparing it with

@@ -4,18 +4,23 @@
 //
 // The weights are stored in tiles of 16 rows by 64 columns, 512 bytes, in the order in which the lanes of a warp want them
 // as the A operand of four m16n8k16 instructions: lane (g, c) has 16 bytes, one word a step, with columns
-// 32 (step / 2) + 8 c + 4 (step % 2) .. + 3 of rows g and g + 8, so that two steps are 32 columns in a row.  Within a word the two values that become one register are 16 bits apart:
+// 32 (step / 2) + 8 c + 4 (step % 2) .. + 3 of rows g and g + 8, so that two steps are 32 columns in a row.  Within a
+// word the two values that become one register are 16 bits apart:
 //   nibble  0 / 4: row g, columns 0 / 1      1 / 5: row g + 8, columns 0 / 1
 //           2 / 6: row g, columns 2 / 3      3 / 7: row g + 8, columns 2 / 3
-// The scales of a tile's 16 rows stand side by side for each group.
+// The scales of a tile's 16 rows stand together for each group, those of rows g and g + 8 side by side.
 //
-// Few rows of x: every weight is read once, half a byte each, and used for at most a few multiplications, so memory is the bound.  The
-// instruction's eight columns are the rows of x; codes become f16 or bf16 exactly (the nibble is put under the exponent of
-// 1024 or 128, and 1032 or 136 is taken off; as bf16 they are 2^-10 of that until the end), and sums are f32 within a group and across groups.  A row of f32 takes three
-// columns: its bf16 parts, which together have its 24 bits.  Operands go straight from global memory into
-// registers; x is small and stays in the first-level cache.  The matrix does not go through tensor memory: for eight
-// columns a tile of 128 rows would have to be converted into shared memory first, and the conversion, not the
+// Few rows of x: every weight is read once, half a byte each, and used for at most a few multiplications, so memory is the
+// bound, and next to it the instructions that turn words into operands (about 65 of f16 and 85 of bf16 for the 16 x 64 weights of a
+// unit; 11008 x 4096 weights are 74 units for each scheduler of the GPU).  The instruction's eight columns are the
+// rows of x; codes become f16 or bf16 exactly, and sums are f32 within a group and across groups.  A row of f32 takes
+// three columns: its bf16 parts, which together have its 24 bits.  The product does not go through tensor memory: for
+// eight columns a tile of 128 rows would have to be converted into shared memory first, and the conversion, not the
 // product, is the work here.
+// One row through 11008 x 4096, groups of 128, f16, recorded: 10.3 us a pass (23 MB; 7 of them in the kernel, 3.5 at the
+// measured rate of memory); 16.5 with a CTA for each row tile, whose first loads, staging of x and sums were not
+// overlapped with anything, and 22 where a scale was converted, and so waited for, in the turn that called for it.
+// Seven rows of bf16 through 4096 x 11008: 14.4 us.
 // Many rows: the weights are written out in the type of x once and the matrix product kernels take them.
 #include <algorithm>
 
@@ -31,7 +36,14 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 16;        // of a CTA of the product; one CTA a SM
+constexpr int kMaxTiles = 32;     // row tiles of a CTA
+constexpr int kSmem = 227 * 1024;
+// A unit, 16 rows by 64 columns, in a warp's ring: its words, and the scales of every lane's two rows
+__host__ __device__ constexpr int ring_unit(bool wide, bool g32) { return 512 + 32 * (wide ? 8 : 4) * (g32 ? 2 : 1); }
+
+// Where the scale of a tile's row is among the 16 of a group
+__host__ __device__ __forceinline__ int scale_slot(int row) { return (row & 7) * 2 + (row >> 3); }
 
 __device__ __forceinline__ float scale_at(const void* s, DType dt, long long i) {
     return dt == DType::F32 ? ((const float*)s)[i] : dt == DType::F16 ? __half2float(((const __half*)s)[i]) : __bfloat162float(((const __nv_bfloat16*)s)[i]);
@@ -78,7 +90,7 @@ __global__ void q4_quantize_kernel(const T* __restrict__ w, long long rs, long l
                 }
                 nib[half][e] = (unsigned)(min(max(code, -8), 7) + 8);
             }
-            if (lane == 0 && q < groups) scales[(rt * groups + q) * 16 + g + half * 8] = st;
+            if (lane == 0 && q < groups) scales[(rt * groups + q) * 16 + scale_slot(g + half * 8)] = st;
         }
         if (active) {
             const long long col = q * group + lane * 4, chunk = col / 64;
@@ -113,7 +125,7 @@ template <typename U>
 __global__ void q4_pack_scales_kernel(const U* __restrict__ in, U* __restrict__ out, long long n, long long groups, long long total) {
     for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
         const long long q = (i >> 4) % groups, row = (i >> 4) / groups * 16 + (i & 15);
-        out[i] = row < n ? in[row * groups + q] : U(0);
+        out[i - (i & 15) + scale_slot((int)(i & 15))] = row < n ? in[row * groups + q] : U(0);
     }
 }
 
@@ -132,7 +144,7 @@ __global__ void q4_dequantize_kernel(const uint32_t* __restrict__ codes, const v
         for (int half = 0; half < 2; ++half) {
             const long long row = rt * 16 + g + half * 8;
             if (row >= n) continue;
-            const float s = scale_at(scales, sdt, (rt * groups + q) * 16 + g + half * 8);
+            const float s = scale_at(scales, sdt, (rt * groups + q) * 16 + scale_slot(g + half * 8));
             Pack<T, 4> v;
 #pragma unroll
             for (int e = 0; e < 4; ++e) v.v[e] = from_f<T>((float)((int)((w >> (4 * nibble(half, e))) & 15u) - 8) * s);
@@ -145,230 +157,411 @@ __global__ void q4_dequantize_kernel(const uint32_t* __restrict__ codes, const v
 }
 
 // ---- few rows --------------------------------------------------------------------------------------------------------
-// Rows of x as the product reads them: columns padded with zeros to whole chunks; a row of f32 as its three bf16 parts.
-template <typename T>
-__global__ void q4_stage_kernel(const T* __restrict__ x, long long rs, long long cs, uint16_t* __restrict__ out, long long rows, long long k, long long kp) {
-    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < rows * kp; i += (long long)gridDim.x * blockDim.x) {
-        const long long r = i / kp, j = i - r * kp;
-        const T v = j < k ? x[r * rs + j * cs] : from_f<T>(0.f);
-        if constexpr (sizeof(T) == 4) {
-            // towards zero, so that no part leaves the range; three parts of 8 bits hold all 24
-            const __nv_bfloat16 a = __float2bfloat16_rz(v);
-            const float r1 = isfinite(v) ? v - __bfloat162float(a) : 0.f;
-            const __nv_bfloat16 b = __float2bfloat16_rz(r1), c = __float2bfloat16_rn(r1 - __bfloat162float(b));
-            out[(r * 3) * kp + j] = __bfloat16_as_ushort(a);
-            out[(r * 3 + 1) * kp + j] = __bfloat16_as_ushort(b);
-            out[(r * 3 + 2) * kp + j] = __bfloat16_as_ushort(c);
-        } else {
-            out[i] = *reinterpret_cast<const uint16_t*>(&v);
-        }
-    }
-}
-
 struct Q4Params {
     const uint4* codes;
     const void* scales;
-    const uint16_t* x;       // [columns][x_stride], 16-byte aligned rows, zeros to the end of the last chunk
+    const void* x;           // [rows][k], last axis dense
     void* y;                 // [rows][n]
-    long long x_stride, n;
-    int columns, rows, parts;    // columns = rows * parts
+    long long x_stride, n, k;
+    int rows, columns;       // columns of the instruction that are in use: one for each row, three for one of f32
     int chunks, groups, group_log2, row_tiles;
     DType scale_dtype;
-    int chunks_per_cta;      // of the CTA's share of the columns
+    int tiles, share_chunks; // row tiles of a cluster, chunks of a CTA's share of them
+    int aligned;             // 16-bit rows of x in 16-byte pieces
 };
 
+// Eight values of a row of x from column `at` on, as one 16-byte operand for each part; zeros behind the end of the row.
+template <typename T> __device__ __forceinline__ void operands(const T* row, long long at, long long k, uint4 (&out)[sizeof(T) == 4 ? 3 : 1]) {
+    T x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = at + e < k ? row[at + e] : from_f<T>(0.f);
+    unsigned short h[sizeof(T) == 4 ? 3 : 1][8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        if constexpr (sizeof(T) == 4) {
+            // the bf16 parts of x: cut towards zero, so that none leaves the range; three of 8 bits hold all 24
+            const __nv_bfloat16 p0 = __float2bfloat16_rz(x[e]);
+            const float r1 = isfinite(x[e]) ? x[e] - __bfloat162float(p0) : 0.f;
+            const __nv_bfloat16 p1 = __float2bfloat16_rz(r1), p2 = __float2bfloat16_rn(r1 - __bfloat162float(p1));
+            h[0][e] = __bfloat16_as_ushort(p0);
+            h[1][e] = __bfloat16_as_ushort(p1);
+            h[2][e] = __bfloat16_as_ushort(p2);
+        } else {
+            h[0][e] = *reinterpret_cast<const unsigned short*>(&x[e]);
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < (sizeof(T) == 4 ? 3 : 1); ++q)
+        out[q] = make_uint4(h[q][0] | (unsigned)h[q][1] << 16, h[q][2] | (unsigned)h[q][3] << 16, h[q][4] | (unsigned)h[q][5] << 16, h[q][6] | (unsigned)h[q][7] << 16);
+}
+
+// The scales of rows g and g + 8, from what a lane's copy brought
+template <bool WIDE> __device__ __forceinline__ float2 two_scales(unsigned at, bool half) {
+    if constexpr (WIDE) return shared_float2(at);
+    const unsigned v = shared_word(at);
+    const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&v));
+    return make_float2(half ? h.x : __uint_as_float(v << 16), half ? h.y : __uint_as_float(v & 0xffff0000u));
+}
+
+// A word's codes as the operand of one instruction.
+// bf16: (code - 8) / 1024, exactly.  x may be anywhere in the range of f32, and sums of 128 products must not leave it.
+// f16: the nibbles where they are, as the smallest numbers of the type: code * 2^-24 in rows g, and 16 times that in rows
+// g + 8, whose nibbles stand four bits higher.  No bit has to move for it but by a shift of eight.  The 8 is taken off by
+// starting the sums from -8 times the sum of x, which is the same for all rows (constant_rows is the operand that gives it),
+// and the powers of two at the end of a stretch.
 template <bool BF> __device__ __forceinline__ void expand(unsigned w, unsigned (&a)[4]) {
     if constexpr (BF) {
-        // (code - 8) / 1024, exactly: x may be anywhere in the range of f32, and sums of 128 products must not leave it
-        const __nv_bfloat162 unit = __halves2bfloat162(__ushort_as_bfloat16(0x3a80), __ushort_as_bfloat16(0x3a80));   // 2^-10
-        const __nv_bfloat162 off = __halves2bfloat162(__ushort_as_bfloat16(0xbe08), __ushort_as_bfloat16(0xbe08));    // -136 * 2^-10
+        const __nv_bfloat162 off = __halves2bfloat162(__ushort_as_bfloat16(0xbe08), __ushort_as_bfloat16(0xbe08));    // -136 / 1024
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const unsigned v = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
-            const __nv_bfloat162 d = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&v), unit, off);
+            const unsigned v = ((w >> (4 * i)) & 0x000f000fu) | 0x3e003e00u;      // (128 + code) / 1024
+            const __nv_bfloat162 d = __hadd2(*reinterpret_cast<const __nv_bfloat162*>(&v), off);
             a[i] = *reinterpret_cast<const unsigned*>(&d);
         }
     } else {
-        // the high nibbles of each byte are 16 (code) above 1024: a sixteenth of that, less 72
-        const __half2 off = __half2half2(__ushort_as_half(0x6408)), sixteenth = __half2half2(__ushort_as_half(0x2c00)), off16 = __half2half2(__ushort_as_half(0xd480));
         const unsigned u = w >> 8;
-        const unsigned v[4] = {(w & 0x000f000fu) | 0x64006400u, (w & 0x00f000f0u) | 0x64006400u, (u & 0x000f000fu) | 0x64006400u, (u & 0x00f000f0u) | 0x64006400u};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const __half2 x = *reinterpret_cast<const __half2*>(&v[i]);
-            const __half2 d = i & 1 ? __hfma2(x, sixteenth, off16) : __hsub2(x, off);
-            a[i] = *reinterpret_cast<const unsigned*>(&d);
-        }
+        a[0] = w & 0x000f000fu;
+        a[1] = w & 0x00f000f0u;
+        a[2] = u & 0x000f000fu;
+        a[3] = u & 0x00f000f0u;
     }
 }
-template <bool BF> __device__ __forceinline__ void mma(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+__device__ __forceinline__ void constant_rows(unsigned (&a)[4]) {
+    a[0] = a[1] = a[2] = a[3] = 0x80088008u;     // -8 * 2^-24
+}
+template <bool BF> __device__ __forceinline__ float upper_unit() { return BF ? 1024.f : 0x1p24f; }    // rows g
+template <bool BF> __device__ __forceinline__ float lower_unit() { return BF ? 1024.f : 0x1p20f; }    // rows g + 8
+
+template <bool BF> __device__ __forceinline__ void mma(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1, bool fresh) {
+    // fresh: the accumulator starts from zero
+    float c[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = fresh ? 0.f : d[i];
     if constexpr (BF)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
     else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 
-// One CTA: TILES row tiles and a share of the columns, which its warps divide chunk by chunk.  The CTAs of a cluster have the
-// shares of the same rows; the first adds them up, in their order.
-template <typename T, bool BF, bool G32, int CT, int TILES>
-__global__ void __launch_bounds__(kWarps * 32) q4_rows_kernel(const __grid_constant__ Q4Params p) {
-    constexpr int NB = 4;                                   // chunks whose words a warp has in flight
+// One CTA has some row tiles and a share of the columns; their (tile, chunk) units in a row are cut into equal stretches for
+// its warps.  A warp has the words and scales of DEPTH units on their way into a ring of its own in shared memory, each
+// lane what it will read itself, the first of them while x is brought there (512 bytes for half a chunk of eight columns, in
+// the order in which lanes read them).  It puts its sums down where a tile or its stretch ends.  The CTAs of a cluster have
+// the shares of the same rows.  Sums are added up in the order of the warps and of the CTAs.
+template <typename T, bool WIDE, bool G32, int CT, int DEPTH>
+__global__ void __launch_bounds__(kWarps * 32, 1) q4_rows_kernel(const __grid_constant__ Q4Params p) {
+    constexpr bool BF = !std::is_same<T, __half>::value;
+    constexpr int PARTS = sizeof(T) == 4 ? 3 : 1;
     constexpr int NS = G32 ? 2 : 1;                         // groups of a chunk that have scales of their own
-    extern __shared__ __align__(16) float sums[];           // [warp][TILES * 16][CT * 8]
+    constexpr int COLS = CT * 8, SLOT = 16 * COLS;
+    constexpr int UNIT = ring_unit(WIDE, G32), SB = WIDE ? 8 : 4;
+    extern __shared__ __align__(16) unsigned char smem[];
+    unsigned char* ring = smem + (threadIdx.x >> 5) * (DEPTH * UNIT);   // [unit]{ 512 bytes of words; the lanes' scales }
+    uint4* xs = reinterpret_cast<uint4*>(smem + kWarps * DEPTH * UNIT); // [chunk][half][column][4], and 16 bytes of zeros
+    float* start = reinterpret_cast<float*>(xs + p.share_chunks * p.columns * 8 + 1);    // f16: [chunk][half][COLS]
+    float* sums = start + (BF ? 0 : p.share_chunks * 2 * COLS);         // [slot][row][column]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     cg::cluster_group cluster = cg::this_cluster();
     const int shares = (int)cluster.num_blocks(), share = (int)cluster.block_rank();
-    const int rt0 = (int)(blockIdx.x / shares) * TILES;
-    const int k0 = share * p.chunks_per_cta, k1 = min(p.chunks, k0 + p.chunks_per_cta);
+    const int rt0 = (int)(blockIdx.x / shares) * p.tiles, tiles = min(p.tiles, p.row_tiles - rt0);
+    const int k0 = share * p.share_chunks, nk = min(p.chunks - k0, p.share_chunks);
+    const int units = tiles * nk, each = (units + kWarps - 1) / kWarps;
+    const int u0 = min(units, warp * each), mine = min(units, u0 + each) - u0;
 
-    float total[TILES][CT][4];
-#pragma unroll
-    for (int t = 0; t < TILES; ++t)
-#pragma unroll
-        for (int n = 0; n < CT; ++n) total[t][n][0] = total[t][n][1] = total[t][n][2] = total[t][n][3] = 0.f;
-
-    const uint4* w[TILES];
-    long long sc[TILES];
-#pragma unroll
-    for (int t = 0; t < TILES; ++t) {
-        const long long rt = min(rt0 + t, p.row_tiles - 1);
-        w[t] = p.codes + rt * p.chunks * 32 + lane;
-        sc[t] = rt * p.groups * 16 + g;
+    // pieces of rows of x, eight values each: copied as they are where they can be
+    const bool copied = sizeof(T) == 2 && p.aligned;
+    if (copied) {
+        for (int m = 0; m < p.rows; ++m) {
+            const T* row = (const T*)p.x + (long long)m * p.x_stride + (long long)k0 * 64;
+            for (int q = threadIdx.x; q < nk * 8; q += kWarps * 32) {
+                uint4* to = xs + ((q >> 2) * p.columns + m) * 4 + (q & 3);
+                if ((long long)k0 * 64 + q * 8 < p.k) copy16(to, row + q * 8);
+                else *to = make_uint4(0, 0, 0, 0);
+            }
+        }
     }
-    const uint16_t* xr[CT];
-    bool have[CT];
+    copies_commit();
+
+    // The unit that is called for next, as offsets from the CTA's first: 16-byte pieces of codes, pairs of scales
+    int tile = u0 / nk, at = u0 - tile * nk, next = k0 + at;
+    const uint4* codes = p.codes + ((long long)rt0 * p.chunks) * 32;
+    const unsigned char* scales = (const unsigned char*)p.scales + (long long)rt0 * p.groups * 8 * SB;
+    unsigned w = (unsigned)(tile * p.chunks + next) * 32 + lane, sc = (unsigned)(tile * p.groups) * 8 + g;
+    const unsigned over = (p.chunks - nk) * 32;             // from the end of a share to the next tile's
+    int left = k0 + nk - next;                              // units of this tile that are still to be called for
+    const int group_shift = p.group_log2 - 6;
+    auto bring = [&](unsigned slot) {
+        copy16_at(slot + lane * 16, codes + w);
+        if constexpr (G32) {
+            copy_at<SB>(slot + 512 + lane * SB, scales + (size_t)(sc + next * 16) * SB);
+            copy_at<SB>(slot + 512 + (32 + lane) * SB, scales + (size_t)(sc + min(next * 2 + 1, p.groups - 1) * 8) * SB);
+        } else {
+            copy_at<SB>(slot + 512 + lane * SB, scales + (size_t)(sc + (next >> group_shift) * 8) * SB);
+        }
+        w += 32;
+        ++next;
+        if (--left == 0) {
+            left = nk;
+            next = k0;
+            w += over;
+            sc += p.groups * 8;
+        }
+    };
+    const unsigned ring0 = shared_address(ring);
+#pragma unroll 4
+    for (int i = 0; i < DEPTH; ++i) {
+        if (i < mine) bring(ring0 + i * UNIT);
+        copies_commit();
+    }
+
+    if (threadIdx.x == 0) xs[nk * 8 * p.columns] = make_uint4(0, 0, 0, 0);
+    if (copied) {
+        copies_wait<DEPTH>();
+    } else {
+        for (int m = 0; m < p.rows; ++m)
+#pragma unroll 2
+            for (int q = threadIdx.x; q < nk * 8; q += kWarps * 32) {
+                uint4 v[PARTS];
+                operands<T>((const T*)p.x + (long long)m * p.x_stride, (long long)k0 * 64 + q * 8, p.k, v);
+#pragma unroll
+                for (int e = 0; e < PARTS; ++e) xs[((q >> 2) * p.columns + m * PARTS + e) * 4 + (q & 3)] = v[e];
+            }
+    }
+    __syncthreads();
+
+    float total[CT][4];
+#pragma unroll
+    for (int n = 0; n < CT; ++n) total[n][0] = total[n][1] = total[n][2] = total[n][3] = 0.f;
+    // a lane whose column of the instruction is not in use reads the zeros behind x, over and over
+    unsigned x0[CT], x_step[CT];
 #pragma unroll
     for (int n = 0; n < CT; ++n) {
-        have[n] = n * 8 + g < p.columns;
-        xr[n] = p.x + (long long)min(n * 8 + g, p.columns - 1) * p.x_stride + c * 8;
+        const bool have = n * 8 + g < p.columns;
+        x0[n] = shared_address(have ? xs + n * 32 + lane : xs + nk * 8 * p.columns);
+        x_step[n] = have ? p.columns * 128 : 0;
     }
-    for (int base = k0 + warp; base < k1; base += kWarps * NB) {
-        uint4 words[NB][TILES];
-        float scale[NB][TILES][NS][2];
+    if constexpr (!BF) {
+        // -8 * 2^-24 times the sums of x over each group of a chunk
+        unsigned a[4];
+        constant_rows(a);
+        for (int k = warp; k < nk; k += kWarps) {
+            float acc[CT][4];
 #pragma unroll
-        for (int i = 0; i < NB; ++i) {
-            const int kc = min(base + i * kWarps, k1 - 1);
+            for (int half = 0; half < 2; ++half)
 #pragma unroll
-            for (int t = 0; t < TILES; ++t) {
-                words[i][t] = __ldcs(w[t] + (long long)kc * 32);
-#pragma unroll
-                for (int q = 0; q < NS; ++q) {
-                    const long long at = sc[t] + (long long)min((kc * 64 + q * 32) >> p.group_log2, p.groups - 1) * 16;
-                    scale[i][t][q][0] = scale_at(p.scales, p.scale_dtype, at);
-                    scale[i][t][q][1] = scale_at(p.scales, p.scale_dtype, at + 8);
+                for (int n = 0; n < CT; ++n) {
+                    const uint4 x = shared_16(x0[n] + k * x_step[n] + (half ? x_step[n] / 2 : 0));
+                    mma<BF>(acc[n], a, x.x, x.y, half == 0 || G32);
+                    mma<BF>(acc[n], a, x.z, x.w, false);
+                    if (g == 0) *reinterpret_cast<float2*>(start + (k * 2 + half) * COLS + n * 8 + c * 2) = make_float2(acc[n][0], acc[n][1]);
                 }
-            }
         }
+        __syncthreads();
+    }
+    const bool half_scales = p.scale_dtype == DType::F16;
+    float* put = sums + (tile + warp) * SLOT + g * COLS + c * 2;       // every (tile, warp) that meet have a slot of their own
+    auto put_down = [&] {
+        const float up = upper_unit<BF>(), low = lower_unit<BF>();
 #pragma unroll
-        for (int i = 0; i < NB; ++i) {
-            const int kc = base + i * kWarps;
-            if (kc < k1) {
-                float acc[TILES][CT][4];
+        for (int n = 0; n < CT; ++n) {
+            *reinterpret_cast<float2*>(put + n * 8) = make_float2(total[n][0] * up, total[n][1] * up);
+            *reinterpret_cast<float2*>(put + 8 * COLS + n * 8) = make_float2(total[n][2] * low, total[n][3] * low);
+            total[n][0] = total[n][1] = total[n][2] = total[n][3] = 0.f;
+        }
+        put += SLOT;
+    };
+    const unsigned ring_end = ring0 + DEPTH * UNIT;
+    unsigned slot = ring0 + lane * 16;
+    int ahead = mine - DEPTH;                               // units still to be called for
+    for (int done = 0; done < mine;) {
+        // a tile's units
+        const int stretch = min(nk - at, mine - done);
+        done += stretch;
+        unsigned xl[CT], from = shared_address(start) + (at * 2 * COLS + c * 2) * 4;
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
+        for (int n = 0; n < CT; ++n) xl[n] = x0[n] + at * x_step[n];
+        at = 0;
+#pragma unroll 2
+        for (int i = 0; i < stretch; ++i) {
+            copies_wait<DEPTH - 1>();
+            const uint4 words = shared_16(slot);
+            float2 s[NS];
+#pragma unroll
+            for (int q = 0; q < NS; ++q) s[q] = two_scales<WIDE>(slot - lane * (16 - SB) + 512 + q * 32 * SB, half_scales);
+            float acc[2][CT][4];                            // the halves of a chunk do not wait for one another
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                uint4 x[CT];
+#pragma unroll
+                for (int n = 0; n < CT; ++n) x[n] = shared_16(xl[n] + (half ? x_step[n] / 2 : 0));
+                if constexpr (!BF) {
+                    // rows g + 8 count in units 16 times as large
                     if (half == 0 || G32) {
 #pragma unroll
-                        for (int t = 0; t < TILES; ++t)
-#pragma unroll
-                            for (int n = 0; n < CT; ++n) acc[t][n][0] = acc[t][n][1] = acc[t][n][2] = acc[t][n][3] = 0.f;
-                    }
-                    uint4 x[CT];
-#pragma unroll
-                    for (int n = 0; n < CT; ++n)
-                        x[n] = have[n] ? __ldg(reinterpret_cast<const uint4*>(xr[n] + (long long)kc * 64 + half * 32)) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-                    for (int t = 0; t < TILES; ++t) {
-                        unsigned a[4];
-                        expand<BF>(half ? words[i][t].z : words[i][t].x, a);
-#pragma unroll
-                        for (int n = 0; n < CT; ++n) mma<BF>(acc[t][n], a, x[n].x, x[n].y);
-                        expand<BF>(half ? words[i][t].w : words[i][t].y, a);
-#pragma unroll
-                        for (int n = 0; n < CT; ++n) mma<BF>(acc[t][n], a, x[n].z, x[n].w);
-                    }
-                    if (half == 1 || G32) {
-#pragma unroll
-                        for (int t = 0; t < TILES; ++t)
-#pragma unroll
-                            for (int n = 0; n < CT; ++n)
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) total[t][n][e] += acc[t][n][e] * scale[i][t][G32 ? half : 0][e >> 1];
+                        for (int n = 0; n < CT; ++n) {
+                            const float2 v = shared_float2(from + ((G32 ? half : 1) * COLS + n * 8) * 4);
+                            acc[half][n][0] = v.x;
+                            acc[half][n][1] = v.y;
+                            acc[half][n][2] = v.x * 16.f;
+                            acc[half][n][3] = v.y * 16.f;
+                        }
                     }
                 }
+                const bool fresh = BF || (half == 1 && !G32);
+                unsigned a[4];
+                expand<BF>(half ? words.z : words.x, a);
+#pragma unroll
+                for (int n = 0; n < CT; ++n) mma<BF>(acc[half][n], a, x[n].x, x[n].y, fresh);
+                expand<BF>(half ? words.w : words.y, a);
+#pragma unroll
+                for (int n = 0; n < CT; ++n) mma<BF>(acc[half][n], a, x[n].z, x[n].w, false);
             }
+            if (ahead > 0) bring(slot - lane * 16);
+            --ahead;
+            copies_commit();
+            slot += UNIT;
+            if (slot >= ring_end) slot -= DEPTH * UNIT;
+#pragma unroll
+            for (int n = 0; n < CT; ++n) xl[n] += x_step[n];
+            from += 2 * COLS * 4;
+#pragma unroll
+            for (int n = 0; n < CT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if constexpr (G32) total[n][e] += acc[0][n][e] * (e < 2 ? s[0].x : s[0].y) + acc[1][n][e] * (e < 2 ? s[1].x : s[1].y);
+                    else total[n][e] += (acc[0][n][e] + acc[1][n][e]) * (e < 2 ? s[0].x : s[0].y);
+                }
         }
+        put_down();
     }
-
-    constexpr int COLS = CT * 8, ROWS = TILES * 16;
-#pragma unroll
-    for (int t = 0; t < TILES; ++t)
-#pragma unroll
-        for (int n = 0; n < CT; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                sums[(warp * ROWS + t * 16 + g + (e >> 1) * 8) * COLS + n * 8 + c * 2 + (e & 1)] = total[t][n][e];
     __syncthreads();
-    // the first warp's place takes the CTA's sum; every value is added up by one thread
-    for (int i = threadIdx.x; i < ROWS * COLS; i += kWarps * 32) {
-        float s = sums[i];
-#pragma unroll
-        for (int v = 1; v < kWarps; ++v) s += sums[v * ROWS * COLS + i];
-        sums[i] = s;
+
+    // What the CTA's warps have of a value, in their order
+    auto warps_sum = [&](int t, int r, int column) {
+        const int w0 = t * nk / each, w1 = ((t + 1) * nk - 1) / each;
+        float s = 0.f;
+        for (int v = w0; v <= w1; ++v) s += sums[((t + v) * 16 + r) * COLS + column];
+        return s;
+    };
+    float* joint = sums + (p.tiles + kWarps) * SLOT;        // [tile][row][column]: this CTA's share
+    if (shares > 1) {
+        for (int i = threadIdx.x; i < tiles * 16 * p.columns; i += kWarps * 32) {
+            const int column = i % p.columns, row = i / p.columns;
+            joint[row * COLS + column] = warps_sum(row >> 4, row & 15, column);
+        }
+        cluster.sync();
     }
-    if (shares > 1) cluster.sync();
-    else __syncthreads();
     if (share == 0) {
-        for (int i = threadIdx.x; i < ROWS * p.rows; i += kWarps * 32) {
-            const int r = i % ROWS, m = i / ROWS;
+        for (int i = threadIdx.x; i < tiles * 16 * p.rows; i += kWarps * 32) {
+            const int r = i % (tiles * 16), m = i / (tiles * 16);
             const long long row = (long long)rt0 * 16 + r;
             if (row >= p.n) continue;
             float y = 0.f;
-            for (int part = p.parts - 1; part >= 0; --part) {       // the smallest part of a row of f32 first
-                const int at = r * COLS + m * p.parts + part;
-                float s = sums[at];
-                for (int v = 1; v < shares; ++v) s += cluster.map_shared_rank(sums, v)[at];
+#pragma unroll
+            for (int q = PARTS - 1; q >= 0; --q) {          // the smallest part of a row of f32 first
+                const int column = m * PARTS + q;
+                float s;
+                if (shares > 1) {
+                    s = joint[r * COLS + column];
+                    for (int v = 1; v < shares; ++v) s += cluster.map_shared_rank(joint, v)[r * COLS + column];
+                } else {
+                    s = warps_sum(r >> 4, r & 15, column);
+                }
                 y += s;
             }
-            ((T*)p.y)[(long long)m * p.n + row] = from_f<T>(BF ? y * 1024.f : y);
+            ((T*)p.y)[(long long)m * p.n + row] = from_f<T>(y);
         }
     }
     if (shares > 1) cluster.sync();                         // nobody leaves while its sums may be read
 }
 
-template <typename T, bool BF, bool G32, int CT, int TILES>
-void launch_rows(Device& dev, const Q4Params& p, int shares) {
-    auto kernel = q4_rows_kernel<T, BF, G32, CT, TILES>;
+// Shared memory of a CTA whose warps have `depth` units on their way
+size_t rows_smem(int share_chunks, int columns, int tiles, int ct, int shares, int unit, int depth) {
+    return (size_t)kWarps * depth * unit + (size_t)share_chunks * (columns * 128 + ct * 64) + 16 +
+           (size_t)(tiles + kWarps + (shares > 1 ? tiles : 0)) * 16 * ct * 8 * sizeof(float);
+}
+
+template <typename T, bool WIDE, bool G32, int CT, int DEPTH>
+void launch_depth(Device& dev, const Q4Params& p, int shares) {
+    auto kernel = q4_rows_kernel<T, WIDE, G32, CT, DEPTH>;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((p.row_tiles + TILES - 1) / TILES * shares));
+    cfg.gridDim = dim3((unsigned)((p.row_tiles + p.tiles - 1) / p.tiles * shares));
     cfg.blockDim = dim3(kWarps * 32);
-    cfg.dynamicSmemBytes = sizeof(float) * kWarps * TILES * 16 * CT * 8;    // 32 KiB at most
+    cfg.dynamicSmemBytes = rows_smem(p.share_chunks, p.columns, p.tiles, CT, shares, ring_unit(WIDE, G32), DEPTH);
     cfg.stream = dev.stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim = {(unsigned)shares, 1, 1};
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = shares > 1 ? 1 : 0;
+    if (!dev.dry) {
+        static unsigned long long done = 0;    // one bit a device; setting it twice does no harm
+        if (dev.ordinal >= 64 || !(done >> dev.ordinal & 1)) {
+            WGF_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+            if (dev.ordinal < 64) done |= 1ull << dev.ordinal;
+        }
+    }
     dev.begin_launch("q4_rows");
     if (!dev.dry) WGF_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
     dev.end_launch();
 }
-template <typename T, bool BF, bool G32>
-void dispatch_rows(Device& dev, const Q4Params& p, int ct, int tiles, int shares) {
-    if (ct == 1 && tiles == 1) launch_rows<T, BF, G32, 1, 1>(dev, p, shares);
-    else if (ct == 1) launch_rows<T, BF, G32, 1, 2>(dev, p, shares);
-    else if (ct == 2 && tiles == 1) launch_rows<T, BF, G32, 2, 1>(dev, p, shares);
-    else if (ct == 2) launch_rows<T, BF, G32, 2, 2>(dev, p, shares);
-    else if (tiles == 1) launch_rows<T, BF, G32, 4, 1>(dev, p, shares);
-    else launch_rows<T, BF, G32, 4, 2>(dev, p, shares);
+// As many units on their way as there is room for
+template <typename T, bool WIDE, bool G32, int CT>
+void launch_rows(Device& dev, const Q4Params& p, int shares) {
+    const int most = (p.tiles * p.share_chunks + kWarps - 1) / kWarps;      // units of a warp
+    if (CT == 1 && most > 8 && rows_smem(p.share_chunks, p.columns, p.tiles, CT, shares, ring_unit(WIDE, G32), 16) <= (size_t)kSmem)
+        launch_depth<T, WIDE, G32, CT, CT == 1 ? 16 : 8>(dev, p, shares);
+    else launch_depth<T, WIDE, G32, CT, 8>(dev, p, shares);
 }
-template <typename T, bool BF>
-void dispatch_group(Device& dev, const Q4Params& p, int ct, int tiles, int shares) {
-    if (p.group_log2 == 5) dispatch_rows<T, BF, true>(dev, p, ct, tiles, shares);
-    else dispatch_rows<T, BF, false>(dev, p, ct, tiles, shares);
+template <typename T>
+void dispatch_rows(Device& dev, const Q4Params& p, int ct, int shares) {
+    auto with = [&](auto wide, auto g32) {
+        constexpr bool WIDE = decltype(wide)::value, G32 = decltype(g32)::value;
+        if (ct == 1) launch_rows<T, WIDE, G32, 1>(dev, p, shares);
+        else if (ct == 2) launch_rows<T, WIDE, G32, 2>(dev, p, shares);
+        else launch_rows<T, WIDE, G32, 4>(dev, p, shares);
+    };
+    const bool wide = p.scale_dtype == DType::F32;
+    if (wide && p.group_log2 == 5) with(std::true_type(), std::true_type());
+    else if (wide) with(std::true_type(), std::false_type());
+    else if (p.group_log2 == 5) with(std::false_type(), std::true_type());
+    else with(std::false_type(), std::false_type());
+}
+
+// How many clusters of 1, 2, 4 and 8 CTAs the GPU runs at once with one CTA a SM: fewer than its SMs would make, as a
+// cluster's SMs have to be neighbours.
+const int* clusters_at_once(Device& dev) {
+    static int known[64][4];
+    int* k = known[dev.dry || dev.ordinal >= 64 ? 63 : dev.ordinal];
+    if (k[0]) return k;
+    k[1] = k[2] = k[3] = 0;
+    for (int i = 1; i < 4; ++i) {
+        k[i] = dev.sm_count >> i;
+        if (dev.dry) continue;
+        auto kernel = q4_rows_kernel<__half, false, false, 1, 8>;
+        WGF_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)(dev.sm_count << i));
+        cfg.blockDim = dim3(kWarps * 32);
+        cfg.dynamicSmemBytes = kSmem;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim = {1u << i, 1, 1};
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        int n = 0;
+        if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+            cudaGetLastError();
+            n = 0;
+        }
+        k[i] = std::max(std::min(n, k[i]), 1);
+    }
+    k[0] = dev.sm_count;
+    return k;
 }
 
 unsigned grid_for(Device& dev, long long items) { return (unsigned)std::min<long long>((items + 255) / 256, (long long)dev.sm_count * 32); }
@@ -479,7 +672,24 @@ TensorData run_matmul_q4(Device& dev, const TensorData& x_in, const Q4Weight& w)
     }
     dev.wait_for(*x.buf);
     const int parts = x.dtype == DType::F32 ? 3 : 1;
-    if (rows * parts > 32) {
+    const int64_t columns = rows * parts;
+    const int ct = columns <= 8 ? 1 : columns <= 16 ? 2 : 4;
+    // How the row tiles are dealt out: to the SMs, or with shares of the columns to clusters of 2, 4 or 8 of them, whichever
+    // leaves the longest CTA the fewest units; joining a cluster's sums is worth about 32.  x has to fit beside the sums.
+    int shares = 0;
+    int64_t best = INT64_MAX, tiles = 0;
+    const int* at_once = clusters_at_once(dev);
+    const int unit = ring_unit(w.scale_dtype == DType::F32, w.group == 32);
+    for (int s = 1, i = 0; i < 4 && columns <= 32; s *= 2, ++i) {
+        const int64_t clusters = at_once[i], t = std::min<int64_t>((w.row_tiles + clusters - 1) / clusters, kMaxTiles);
+        const int64_t turns = ((w.row_tiles + t - 1) / t + clusters - 1) / clusters, chunks = (w.chunks + s - 1) / s;
+        const int64_t cost = turns * t * chunks + (s > 1 ? 32 : 0);
+        if ((s - 1) * chunks >= w.chunks || cost >= best || rows_smem((int)chunks, (int)columns, (int)t, ct, s, unit, 8) > (size_t)kSmem) continue;
+        best = cost;
+        shares = s;
+        tiles = t;
+    }
+    if (!shares) {
         TensorData full = q4_dequantize(dev, w, x.dtype);
         full.layout.shape = {w.k, w.n};
         full.layout.strides = {1, w.k};
@@ -489,46 +699,29 @@ TensorData run_matmul_q4(Device& dev, const TensorData& x_in, const Q4Weight& w)
     }
     dev.note_recorded_buffer(w.codes);
     dev.note_recorded_buffer(w.scales);
+    if (x.layout.strides[1] != 1 && w.k > 1) x = run_compact(dev, x);
     out.buf = dev.alloc((size_t)(rows * w.n) * dtype_size(x.dtype), false);
     Q4Params p{};
     p.codes = (const uint4*)w.codes->ptr;
     p.scales = w.scales->ptr;
+    p.x = x.base_ptr();
+    p.x_stride = x.layout.strides[0];
     p.y = out.buf->ptr;
     p.n = w.n;
+    p.k = w.k;
     p.rows = (int)rows;
-    p.parts = parts;
-    p.columns = (int)rows * parts;
+    p.columns = (int)columns;
     p.chunks = (int)w.chunks;
     p.groups = (int)w.groups;
     p.group_log2 = w.group == 32 ? 5 : w.group == 64 ? 6 : 7;
     p.row_tiles = (int)w.row_tiles;
     p.scale_dtype = w.scale_dtype;
-    BufferRef staged;
-    if (parts == 1 && w.k % 64 == 0 && x.layout.strides[1] == 1 && (rows == 1 || x.layout.strides[0] % 8 == 0) && (uintptr_t)x.base_ptr() % 16 == 0) {
-        p.x = (const uint16_t*)x.base_ptr();
-        p.x_stride = x.layout.strides[0];
-    } else {
-        const long long kp = w.chunks * 64;
-        staged = dev.alloc((size_t)(p.columns * kp) * 2, false);
-        p.x = (const uint16_t*)staged->ptr;
-        p.x_stride = kp;
-        dev.begin_launch("q4_stage");
-        if (!dev.dry) {
-            const unsigned grid = grid_for(dev, rows * kp);
-            if (x.dtype == DType::F32) q4_stage_kernel<float><<<grid, 256, 0, dev.stream>>>((const float*)x.base_ptr(), x.layout.strides[0], x.layout.strides[1], (uint16_t*)staged->ptr, rows, w.k, kp);
-            else q4_stage_kernel<__half><<<grid, 256, 0, dev.stream>>>((const __half*)x.base_ptr(), x.layout.strides[0], x.layout.strides[1], (uint16_t*)staged->ptr, rows, w.k, kp);
-        }
-        dev.end_launch();
-    }
-    const int ct = p.columns <= 8 ? 1 : p.columns <= 16 ? 2 : 4;
-    const int tiles = 1;
-    // CTAs for the whole GPU, as long as each warp has a chunk
-    int shares = 1;
-    while (shares < 8 && (w.row_tiles / tiles) * shares < 2 * dev.sm_count && w.chunks / (shares * 2) >= kWarps) shares *= 2;
-    p.chunks_per_cta = (int)((w.chunks + shares - 1) / shares);
-    if (x.dtype == DType::F16) dispatch_group<__half, false>(dev, p, ct, tiles, shares);
-    else if (x.dtype == DType::BF16) dispatch_group<__nv_bfloat16, true>(dev, p, ct, tiles, shares);
-    else dispatch_group<float, true>(dev, p, ct, tiles, shares);
+    p.tiles = (int)tiles;
+    p.share_chunks = (int)((w.chunks + shares - 1) / shares);
+    p.aligned = parts == 1 && w.k % 8 == 0 && (rows == 1 || p.x_stride % 8 == 0) && (uintptr_t)p.x % 16 == 0;
+    if (x.dtype == DType::F32) dispatch_rows<float>(dev, p, ct, shares);
+    else if (x.dtype == DType::F16) dispatch_rows<__half>(dev, p, ct, shares);
+    else dispatch_rows<__nv_bfloat16>(dev, p, ct, shares);
     return out;
 }
 
