@@ -555,9 +555,9 @@ extern "C" {
     ) -> i32;
     /// The values as a [n, k] tensor of `dtype`.
     pub fn wgf_q4_weight_dequantize(w: *mut wgf_q4_weight, dtype: u32, out: *mut *mut wgf_tensor) -> i32;
-    /// x [.., k] times the transposed weights: [.., n] of x's type, lazily.  A few rows are one kernel that
-    /// reads the codes, with f32 sums of exact products; for many rows the weights are first written
-    /// out in x's type (their values rounded to it) and the matrix product runs on them.
+    /// x [.., k] times the transposed weights: [.., n] of x's type, lazily.  Up to some dozens of rows
+    /// are one kernel that reads the codes, with f32 sums of exact products; for more the weights are
+    /// first written out in x's type (their values rounded to it) and the matrix product runs on them.
     pub fn wgf_tensor_matmul_q4(x: *mut wgf_tensor, w: *mut wgf_q4_weight, out: *mut *mut wgf_tensor) -> i32;
     /// Contiguous block partition of `n_units` over `world` ranks: the first n_units % world
     /// ranks get one extra unit.

@@ -372,6 +372,21 @@ def test_q4_product(kind, rows, n, k, group, wgf, dev):
     close(out, *ref.q4_product(x, ref.q4_values(c, s, group), kind, through=None if rows <= 8 else kind))
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows,n,k,group,written_out", [(700, 72, 64, 32, ["f32"]), (3001, 130, 70, 32, ["f32"]), (200, 40, 300, 128, []), (65, 300, 1100, 64, []),
+                                                        (600, 1500, 2100, 64, KINDS)])
+def test_q4_product_of_many_rows(kind, rows, n, k, group, written_out, wgf, dev):
+    """Rows in blocks, and weights that are written out for the matrix product, in padded rows where k is odd for it."""
+    g = seeded(23, rows)
+    w, x = draw(g, (n, k), kind, 0.02), draw(g, (rows, k), kind)
+    c, s = ref.q4_quantize(w, group, kind)
+    t = give(wgf, dev, w, kind).quantize_q4(group)
+    dev.set_timing(True)
+    out = give(wgf, dev, x, kind).mat_mul_q4(t)
+    close(take(out, kind), *ref.q4_product(x, ref.q4_values(c, s, group), kind, through=kind if kind in written_out else None))
+    assert ("q4_dequantize" in out.timing_labels()) == (kind in written_out)
+
+
 @pytest.mark.parametrize("kind", ["f32", "f16"])
 def test_q4_product_of_views_and_ranks(kind, wgf, dev):
     g = seeded(23, 77)

@@ -21,7 +21,8 @@
 // measured rate of memory); 16.5 with a CTA for each row tile, whose first loads, staging of x and sums were not
 // overlapped with anything, and 22 where a scale was converted, and so waited for, in the turn that called for it.
 // Seven rows of bf16 through 4096 x 11008: 14.4 us.
-// Many rows: the weights are written out in the type of x once and the matrix product kernels take them.
+// More rows: in blocks, along the grid's second axis.  Many rows: the weights are written out in the type of x once and
+// the matrix product kernels take them (rows_in_blocks has both sides' times).
 #include <algorithm>
 
 #include <cooperative_groups.h>
@@ -132,14 +133,14 @@ __global__ void q4_pack_scales_kernel(const U* __restrict__ in, U* __restrict__ 
 // The values that the codes stand for, row by row.  A thread has one word: four columns of two rows.
 template <typename T>
 __global__ void q4_dequantize_kernel(const uint32_t* __restrict__ codes, const void* __restrict__ scales, DType sdt, T* __restrict__ out, long long n,
-                                     long long k, int group, long long chunks, long long groups, long long words) {
+                                     long long k, long long stride, int group, long long chunks, long long groups, long long words) {
     for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < words; i += (long long)gridDim.x * blockDim.x) {
         // neighbours write neighbouring columns
         const int c = (int)(i >> 1) & 3, st = (int)(i >> 3 & 1) * 2 + (int)(i & 1), g = (int)(i >> 4) & 7;
         const long long tile = i >> 7, rt = tile / chunks, col = (tile % chunks) * 64 + (i & 15) * 4;
         const unsigned w = codes[tile * 128 + (g * 4 + c) * 4 + st];
-        if (col >= k) continue;
-        const long long q = col / group;
+        if (col >= stride) continue;                        // zeros between the last column and the end of a padded row
+        const long long q = min(col / group, groups - 1);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             const long long row = rt * 16 + g + half * 8;
@@ -147,11 +148,11 @@ __global__ void q4_dequantize_kernel(const uint32_t* __restrict__ codes, const v
             const float s = scale_at(scales, sdt, (rt * groups + q) * 16 + scale_slot(g + half * 8));
             Pack<T, 4> v;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v.v[e] = from_f<T>((float)((int)((w >> (4 * nibble(half, e))) & 15u) - 8) * s);
-            T* to = out + row * k + col;
-            if (k % 4 == 0) *reinterpret_cast<Pack<T, 4>*>(to) = v;
+            for (int e = 0; e < 4; ++e) v.v[e] = from_f<T>(col + e < k ? (float)((int)((w >> (4 * nibble(half, e))) & 15u) - 8) * s : 0.f);
+            T* to = out + row * stride + col;
+            if (stride % 4 == 0) *reinterpret_cast<Pack<T, 4>*>(to) = v;
             else
-                for (int e = 0; e < 4 && col + e < k; ++e) to[e] = v.v[e];
+                for (int e = 0; e < 4 && col + e < stride; ++e) to[e] = v.v[e];
         }
     }
 }
@@ -163,7 +164,8 @@ struct Q4Params {
     const void* x;           // [rows][k], last axis dense
     void* y;                 // [rows][n]
     long long x_stride, n, k;
-    int rows, columns;       // columns of the instruction that are in use: one for each row, three for one of f32
+    int rows, columns;       // of a block of rows; columns of the instruction: one for each row, three for one of f32
+    int all_rows;            // blocks of rows lie along the grid's second axis
     int chunks, groups, group_log2, row_tiles;
     DType scale_dtype;
     int tiles, share_chunks; // row tiles of a cluster, chunks of a CTA's share of them
@@ -269,14 +271,16 @@ __global__ void __launch_bounds__(kWarps * 32, 1) q4_rows_kernel(const __grid_co
     const int shares = (int)cluster.num_blocks(), share = (int)cluster.block_rank();
     const int rt0 = (int)(blockIdx.x / shares) * p.tiles, tiles = min(p.tiles, p.row_tiles - rt0);
     const int k0 = share * p.share_chunks, nk = min(p.chunks - k0, p.share_chunks);
+    const T* x_rows = (const T*)p.x + (long long)blockIdx.y * p.rows * p.x_stride;
+    const int rows = min(p.rows, p.all_rows - (int)blockIdx.y * p.rows);
     const int units = tiles * nk, each = (units + kWarps - 1) / kWarps;
     const int u0 = min(units, warp * each), mine = min(units, u0 + each) - u0;
 
     // pieces of rows of x, eight values each: copied as they are where they can be
     const bool copied = sizeof(T) == 2 && p.aligned;
     if (copied) {
-        for (int m = 0; m < p.rows; ++m) {
-            const T* row = (const T*)p.x + (long long)m * p.x_stride + (long long)k0 * 64;
+        for (int m = 0; m < rows; ++m) {
+            const T* row = x_rows + (long long)m * p.x_stride + (long long)k0 * 64;
             for (int q = threadIdx.x; q < nk * 8; q += kWarps * 32) {
                 uint4* to = xs + ((q >> 2) * p.columns + m) * 4 + (q & 3);
                 if ((long long)k0 * 64 + q * 8 < p.k) copy16(to, row + q * 8);
@@ -322,11 +326,11 @@ __global__ void __launch_bounds__(kWarps * 32, 1) q4_rows_kernel(const __grid_co
     if (copied) {
         copies_wait<DEPTH>();
     } else {
-        for (int m = 0; m < p.rows; ++m)
+        for (int m = 0; m < rows; ++m)
 #pragma unroll 2
             for (int q = threadIdx.x; q < nk * 8; q += kWarps * 32) {
                 uint4 v[PARTS];
-                operands<T>((const T*)p.x + (long long)m * p.x_stride, (long long)k0 * 64 + q * 8, p.k, v);
+                operands<T>(x_rows + (long long)m * p.x_stride, (long long)k0 * 64 + q * 8, p.k, v);
 #pragma unroll
                 for (int e = 0; e < PARTS; ++e) xs[((q >> 2) * p.columns + m * PARTS + e) * 4 + (q & 3)] = v[e];
             }
@@ -340,7 +344,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) q4_rows_kernel(const __grid_co
     unsigned x0[CT], x_step[CT];
 #pragma unroll
     for (int n = 0; n < CT; ++n) {
-        const bool have = n * 8 + g < p.columns;
+        const bool have = n * 8 + g < rows * PARTS;
         x0[n] = shared_address(have ? xs + n * 32 + lane : xs + nk * 8 * p.columns);
         x_step[n] = have ? p.columns * 128 : 0;
     }
@@ -455,26 +459,25 @@ __global__ void __launch_bounds__(kWarps * 32, 1) q4_rows_kernel(const __grid_co
         }
         cluster.sync();
     }
-    if (share == 0) {
-        for (int i = threadIdx.x; i < tiles * 16 * p.rows; i += kWarps * 32) {
-            const int r = i % (tiles * 16), m = i / (tiles * 16);
-            const long long row = (long long)rt0 * 16 + r;
-            if (row >= p.n) continue;
-            float y = 0.f;
+    // with shares, each CTA of the cluster adds up a part of the values
+    for (int i = threadIdx.x + share * (kWarps * 32); i < tiles * 16 * rows; i += kWarps * 32 * shares) {
+        const int r = i % (tiles * 16), m = i / (tiles * 16);
+        const long long row = (long long)rt0 * 16 + r;
+        if (row >= p.n) continue;
+        float y = 0.f;
 #pragma unroll
-            for (int q = PARTS - 1; q >= 0; --q) {          // the smallest part of a row of f32 first
-                const int column = m * PARTS + q;
-                float s;
-                if (shares > 1) {
-                    s = joint[r * COLS + column];
-                    for (int v = 1; v < shares; ++v) s += cluster.map_shared_rank(joint, v)[r * COLS + column];
-                } else {
-                    s = warps_sum(r >> 4, r & 15, column);
-                }
-                y += s;
+        for (int q = PARTS - 1; q >= 0; --q) {              // the smallest part of a row of f32 first
+            const int column = m * PARTS + q;
+            float s = 0.f;
+            if (shares > 1) {
+#pragma unroll 2
+                for (int v = 0; v < shares; ++v) s += cluster.map_shared_rank(joint, v)[r * COLS + column];
+            } else {
+                s = warps_sum(r >> 4, r & 15, column);
             }
-            ((T*)p.y)[(long long)m * p.n + row] = from_f<T>(y);
+            y += s;
         }
+        ((T*)p.y)[((long long)blockIdx.y * p.rows + m) * p.n + row] = from_f<T>(y);
     }
     if (shares > 1) cluster.sync();                         // nobody leaves while its sums may be read
 }
@@ -489,7 +492,7 @@ template <typename T, bool WIDE, bool G32, int CT, int DEPTH>
 void launch_depth(Device& dev, const Q4Params& p, int shares) {
     auto kernel = q4_rows_kernel<T, WIDE, G32, CT, DEPTH>;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((p.row_tiles + p.tiles - 1) / p.tiles * shares));
+    cfg.gridDim = dim3((unsigned)((p.row_tiles + p.tiles - 1) / p.tiles * shares), (unsigned)((p.all_rows + p.rows - 1) / p.rows));
     cfg.blockDim = dim3(kWarps * 32);
     cfg.dynamicSmemBytes = rows_smem(p.share_chunks, p.columns, p.tiles, CT, shares, ring_unit(WIDE, G32), DEPTH);
     cfg.stream = dev.stream;
@@ -522,8 +525,7 @@ void dispatch_rows(Device& dev, const Q4Params& p, int ct, int shares) {
     auto with = [&](auto wide, auto g32) {
         constexpr bool WIDE = decltype(wide)::value, G32 = decltype(g32)::value;
         if (ct == 1) launch_rows<T, WIDE, G32, 1>(dev, p, shares);
-        else if (ct == 2) launch_rows<T, WIDE, G32, 2>(dev, p, shares);
-        else launch_rows<T, WIDE, G32, 4>(dev, p, shares);
+        else launch_rows<T, WIDE, G32, 2>(dev, p, shares);
     };
     const bool wide = p.scale_dtype == DType::F32;
     if (wide && p.group_log2 == 5) with(std::true_type(), std::true_type());
@@ -630,27 +632,70 @@ Q4Ref q4_from_host(const DeviceRef& devref, int64_t n, int64_t k, int64_t group,
     return w;
 }
 
-TensorData q4_dequantize(Device& dev, const Q4Weight& w, DType dtype) {
+// [n, k] in rows of `stride` elements, zeros behind the last column
+static TensorData dequantize_rows(Device& dev, const Q4Weight& w, DType dtype, int64_t stride) {
     dev.make_current();
     dev.note_recorded_buffer(w.codes);
     dev.note_recorded_buffer(w.scales);
     TensorData out;
     out.dtype = dtype;
-    out.layout = Layout::contiguous({w.n, w.k});
-    out.buf = dev.alloc((size_t)(w.n * w.k) * dtype_size(dtype), false);
+    out.layout = Layout::contiguous({w.n, stride});
+    out.buf = dev.alloc((size_t)(w.n * stride) * dtype_size(dtype), false);
     const long long words = w.row_tiles * w.chunks * 128;
     auto go = [&](auto zero) {
         typedef decltype(zero) T;
         dev.begin_launch("q4_dequantize");
         if (!dev.dry)
             q4_dequantize_kernel<T><<<grid_for(dev, words), 256, 0, dev.stream>>>((const uint32_t*)w.codes->ptr, w.scales->ptr, w.scale_dtype,
-                (T*)out.buf->ptr, w.n, w.k, (int)w.group, w.chunks, w.groups, words);
+                (T*)out.buf->ptr, w.n, w.k, stride, (int)w.group, w.chunks, w.groups, words);
         dev.end_launch();
     };
     if (dtype == DType::F32) go(0.f);
     else if (dtype == DType::F16) go(__half());
     else go(__nv_bfloat16());
     return out;
+}
+
+TensorData q4_dequantize(Device& dev, const Q4Weight& w, DType dtype) { return dequantize_rows(dev, w, dtype, w.k); }
+
+// How the product with few rows is dealt out: rows in blocks, row tiles of the weights to the SMs, or with shares of the
+// columns to clusters of them.  x has to fit beside the sums.
+struct RowsPlan {
+    int shares = 0, tiles = 0, ct = 0, block_rows = 0;     // shares == 0: it does not fit
+    double cost = 1e30;                                    // in the time that a SM takes for a unit with eight columns, about 21 ns
+};
+static RowsPlan plan_rows(Device& dev, const Q4Weight& w, int64_t rows, int parts) {
+    RowsPlan best;
+    const int* at_once = clusters_at_once(dev);
+    const int unit = ring_unit(w.scale_dtype == DType::F32, w.group == 32);
+    // Joining a cluster's sums costs more than it saves from clusters of four on (eight rows of f16 through 11008 x 4096: 21 us
+    // with four, 13 with one), so those are for rows of x that fit in no other way.
+    for (int s = 1, i = 0; i < 4 && (i < 2 || !best.shares); s *= 2, ++i)
+        for (int ct : {1, 2}) {
+            const int64_t most = ct * 8 / parts, blocks = (rows + most - 1) / most, block_rows = (rows + blocks - 1) / blocks, columns = block_rows * parts;
+            if (blocks > 65535 || (ct == 2 && columns <= 8)) continue;
+            const int64_t chunks = (w.chunks + s - 1) / s, clusters = at_once[i];
+            const int64_t room = (int64_t)kSmem - (int64_t)rows_smem((int)std::min<int64_t>(chunks, 1 << 20), (int)columns, 0, ct, s, unit, 8);
+            const int64_t fit = room / ((s > 1 ? 2 : 1) * 16 * ct * 8 * (int64_t)sizeof(float));      // tiles whose sums there is room for
+            if ((s - 1) * chunks >= w.chunks || fit < 1) continue;
+            const int64_t t = std::min<int64_t>({(w.row_tiles * blocks + clusters - 1) / clusters, w.row_tiles, fit, kMaxTiles});
+            const int64_t turns = ((w.row_tiles + t - 1) / t * blocks + clusters - 1) / clusters;
+            // the units, the bringing of x, what a CTA costs at its ends; and the joining
+            const double cost = (double)turns * ((double)chunks * (t * (ct == 1 ? 1.0 : 1.4) + 0.13 * columns) + 40) + (s > 1 ? 40 + 0.8 * t * columns : 0);
+            if (cost < best.cost) best = {s, (int)t, ct, (int)block_rows, cost};
+        }
+    return best;
+}
+
+// Whether rows go through the kernel above in blocks, or through weights that are written out and the matrix product.
+// Rows of 16 bits: the tensor-core product takes 64 rows at least (fewer run strided: 640 us for 16 rows through
+// 11008 x 4096, 19 in blocks); from there on both sides are estimated.  In us, blocks against weights written out:
+// 11008 x 4096: 80 rows 76 / 80, 100 rows 82 / 80; 4096 x 4096: 80 rows 27 / 43, 128 rows 56 / 43; 600 x 900: 200 rows 13 / 19.
+// Rows of f32: the FFMA product is slow for rows like these: 4096 x 4096: 500 rows 501 / 615; 11008 x 4096: 500 rows 1308 / 1562.
+static bool rows_in_blocks(const RowsPlan& plan, const Q4Weight& w, int64_t rows, int parts) {
+    if (!plan.shares) return false;
+    if (parts > 1) return rows <= 512;
+    return rows < 64 || 3.0 + 0.021 * plan.cost < 12.0 + 0.005 * (double)w.k + 1.1e-6 * (double)w.n * (double)w.k;
 }
 
 TensorData run_matmul_q4(Device& dev, const TensorData& x_in, const Q4Weight& w) {
@@ -672,27 +717,23 @@ TensorData run_matmul_q4(Device& dev, const TensorData& x_in, const Q4Weight& w)
     }
     dev.wait_for(*x.buf);
     const int parts = x.dtype == DType::F32 ? 3 : 1;
-    const int64_t columns = rows * parts;
-    const int ct = columns <= 8 ? 1 : columns <= 16 ? 2 : 4;
-    // How the row tiles are dealt out: to the SMs, or with shares of the columns to clusters of 2, 4 or 8 of them, whichever
-    // leaves the longest CTA the fewest units; joining a cluster's sums is worth about 32.  x has to fit beside the sums.
-    int shares = 0;
-    int64_t best = INT64_MAX, tiles = 0;
-    const int* at_once = clusters_at_once(dev);
-    const int unit = ring_unit(w.scale_dtype == DType::F32, w.group == 32);
-    for (int s = 1, i = 0; i < 4 && columns <= 32; s *= 2, ++i) {
-        const int64_t clusters = at_once[i], t = std::min<int64_t>((w.row_tiles + clusters - 1) / clusters, kMaxTiles);
-        const int64_t turns = ((w.row_tiles + t - 1) / t + clusters - 1) / clusters, chunks = (w.chunks + s - 1) / s;
-        const int64_t cost = turns * t * chunks + (s > 1 ? 32 : 0);
-        if ((s - 1) * chunks >= w.chunks || cost >= best || rows_smem((int)chunks, (int)columns, (int)t, ct, s, unit, 8) > (size_t)kSmem) continue;
-        best = cost;
-        shares = s;
-        tiles = t;
-    }
-    if (!shares) {
-        TensorData full = q4_dequantize(dev, w, x.dtype);
-        full.layout.shape = {w.k, w.n};
-        full.layout.strides = {1, w.k};
+    const RowsPlan plan = plan_rows(dev, w, rows, parts);
+    if (!rows_in_blocks(plan, w, rows, parts)) {
+        // in rows of whole 16 bytes, which the tensor-core kernels want of both operands
+        const int64_t kp = parts == 1 ? (w.k + 7) / 8 * 8 : w.k;
+        TensorData full = dequantize_rows(dev, w, x.dtype, kp);
+        if (kp != w.k) {
+            TensorData wide;
+            wide.dtype = x.dtype;
+            wide.layout = Layout::contiguous({rows, kp});
+            wide.buf = dev.alloc((size_t)(rows * kp) * dtype_size(x.dtype), true);
+            TensorData window = wide;
+            window.layout.shape = {rows, w.k};
+            run_copy(dev, window, x);
+            x = wide;
+        }
+        full.layout.shape = {kp, w.n};
+        full.layout.strides = {1, kp};
         TensorData y = run_matmul(dev, x, full);
         y.layout = out.layout;
         return y;
@@ -709,19 +750,20 @@ TensorData run_matmul_q4(Device& dev, const TensorData& x_in, const Q4Weight& w)
     p.y = out.buf->ptr;
     p.n = w.n;
     p.k = w.k;
-    p.rows = (int)rows;
-    p.columns = (int)columns;
+    p.rows = plan.block_rows;
+    p.all_rows = (int)rows;
+    p.columns = plan.block_rows * parts;
     p.chunks = (int)w.chunks;
     p.groups = (int)w.groups;
     p.group_log2 = w.group == 32 ? 5 : w.group == 64 ? 6 : 7;
     p.row_tiles = (int)w.row_tiles;
     p.scale_dtype = w.scale_dtype;
-    p.tiles = (int)tiles;
-    p.share_chunks = (int)((w.chunks + shares - 1) / shares);
+    p.tiles = plan.tiles;
+    p.share_chunks = (int)((w.chunks + plan.shares - 1) / plan.shares);
     p.aligned = parts == 1 && w.k % 8 == 0 && (rows == 1 || p.x_stride % 8 == 0) && (uintptr_t)p.x % 16 == 0;
-    if (x.dtype == DType::F32) dispatch_rows<float>(dev, p, ct, shares);
-    else if (x.dtype == DType::F16) dispatch_rows<__half>(dev, p, ct, shares);
-    else dispatch_rows<__nv_bfloat16>(dev, p, ct, shares);
+    if (x.dtype == DType::F32) dispatch_rows<float>(dev, p, plan.ct, plan.shares);
+    else if (x.dtype == DType::F16) dispatch_rows<__half>(dev, p, plan.ct, plan.shares);
+    else dispatch_rows<__nv_bfloat16>(dev, p, plan.ct, plan.shares);
     return out;
 }
 
