@@ -35,6 +35,7 @@ namespace {
 
 constexpr int kBlock = KvCache::kBlock;
 constexpr int kWarps = 4;
+constexpr int kGiven = 256;
 constexpr int kRows = 8;        // query rows of a tile
 constexpr int kMaxBatch = 1024; // sequences whose work is shared out evenly
 constexpr int kStages = 3;      // half blocks (keys or values of 64 tokens) in a warp's ring
@@ -52,6 +53,7 @@ struct AttParams {
     int rows, tiles;       // rows of a kv head, tiles of eight of them
     int whole;             // one CTA for each job
     float scale_log2;
+    int given[kGiven];     // counts of a small batch (use_counts == 2; 1: in the second half of lens)
 };
 
 __device__ __forceinline__ unsigned pair_f16(float a, float b) {
@@ -83,15 +85,17 @@ __device__ __forceinline__ void mma(float (&c)[4], unsigned a0, unsigned a1, uns
 template <int DP> constexpr size_t ring_bytes() { return (size_t)kWarps * kStages * kBlock * DP; }
 template <int DP> constexpr size_t att_smem() { return ring_bytes<DP>() + (size_t)DP / 64 * 4 * 512 + kRows * 8; }
 
-// Fills before[0 .. batch] with running sums of the sequences' quads (four blocks, one for each warp; at least one, for the
-// zeros of an empty sequence) and returns the last.
-__device__ __forceinline__ int scan_quads(const AttParams& p, int* before) {
+// Quads (four blocks, one for each warp) of a sequence; at least one, for the zeros of an empty sequence
+__device__ __forceinline__ int quads_of(const AttParams& p, int b) { return max((p.lens[b] + kWarps * kBlock - 1) / (kWarps * kBlock), 1); }
+
+// Fills before[0 .. batch] with running sums of the sequences' quads in pieces of `share` and returns the last.
+__device__ __forceinline__ int scan_quads(const AttParams& p, int* before, int share) {
     __shared__ int sums[kWarps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int run = 0;
     for (int b0 = 0; b0 < p.batch; b0 += kWarps * 32) {
         const int b = b0 + threadIdx.x;
-        int x = b < p.batch ? max((p.lens[b] + kWarps * kBlock - 1) / (kWarps * kBlock), 1) : 0;
+        int x = b < p.batch ? (quads_of(p, b) + share - 1) / share : 0;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
             const int y = __shfl_up_sync(0xffffffffu, x, d);
@@ -108,13 +112,19 @@ __device__ __forceinline__ int scan_quads(const AttParams& p, int* before) {
     __syncthreads();
     return run;
 }
+// How many pieces of `share` quads all sequences have; every warp adds them up for itself.
+__device__ __forceinline__ int pieces_of(const AttParams& p, const int* before, int share) {
+    int n = 0;
+    for (int b = threadIdx.x & 31; b < p.batch; b += 32) n += (before[b + 1] - before[b] + share - 1) / share;
+    return __reduce_add_sync(0xffffffffu, n);
+}
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(kWarps * 32) cache_attention_kernel(const __grid_constant__ AttParams p) {
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ unsigned last;
     __shared__ float total[kRows];
-    __shared__ int before[kMaxBatch + 1];                        // quads of a head's tile in the sequences before
+    __shared__ int before[kMaxBatch + 1];                        // quads, or pieces, of a head's tile in the sequences before
     constexpr int NJ = DP / 64;      // chunks of 64 dims
     constexpr int ND = DP / 8;       // groups of 8 dims
     constexpr int kPart = 2 * kRows + kRows * DP;
@@ -122,13 +132,24 @@ __global__ void __launch_bounds__(kWarps * 32) cache_attention_kernel(const __gr
     unsigned char* ring = smem + warp * (kStages * kBlock * DP) + lane * 16;
     const long long ht = (long long)p.heads * p.tiles;
 
-    // This CTA's share of all quads: [at, stop).  With `whole`, one job's.
+    // This CTA's share of all quads: [at, stop).  A job's end within a share costs about as much as two quads, so where
+    // there are enough CTAs for short shares that end with their jobs, and are at most two quads longer, they do (`pieces`:
+    // `at` then counts pieces).  With `whole`, one job's.
     long long at = 0, stop = 1, share = 1;
+    bool pieces = false;
     if (!p.whole) {
-        const long long all = ht * scan_quads(p, before);
+        const long long all = ht * scan_quads(p, before, 1);
         share = (all + gridDim.x - 1) / gridDim.x;
-        at = (long long)blockIdx.x * share;
-        stop = min(all, at + share);
+        for (int longer = 0; longer < 3 && !pieces && share > 1 && share <= 16; ++longer) pieces = ht * pieces_of(p, before, (int)share + longer) <= gridDim.x && (share += longer, true);
+        if (pieces) {
+            __syncthreads();
+            const long long n = ht * scan_quads(p, before, (int)share);
+            at = blockIdx.x;
+            stop = min(n, at + 1);
+        } else {
+            at = (long long)blockIdx.x * share;
+            stop = min(all, at + share);
+        }
     }
     const long long first = at;
     while (at < stop) {
@@ -154,15 +175,16 @@ __global__ void __launch_bounds__(kWarps * 32) cache_attention_kernel(const __gr
         const int h = (int)(hj / p.tiles), tile = (int)(hj - (long long)h * p.tiles);
         const long long bh = (long long)b * p.heads + h, job = b * ht + hj;
         const long long seg = p.whole ? quads : min(stop, job_at + quads) - at;
+        const long long scale_up = pieces ? share : 1;               // quads of a unit of `at`
         const int len = p.lens[b];
-        const int count = p.use_counts ? p.lens[p.batch + b] : p.t;
+        const int count = p.use_counts == 2 ? p.given[b] : p.use_counts ? p.lens[p.batch + b] : p.t;
         // how many keys a row may see: those up to its own position
         auto limit = [&](int row) {
             const int i = row % p.t;
             return row < p.rows && i < count ? max(len - count + i + 1, 0) : 0;
         };
         const int nblk = (len + kBlock - 1) / kBlock;
-        const int begin = (int)min((at - job_at) * kWarps, (long long)nblk), end = (int)min((at - job_at + seg) * kWarps, (long long)nblk);
+        const int begin = (int)min((at - job_at) * scale_up * kWarps, (long long)nblk), end = (int)min((at - job_at + seg) * scale_up * kWarps, (long long)nblk);
 
         const uint8_t* base = p.codes + bh * p.blocks * (2ll * kBlock * DP);
         // half block n of this warp: block begin + warp + (n / 2) * 4, keys (n even) or values
@@ -320,7 +342,8 @@ __global__ void __launch_bounds__(kWarps * 32) cache_attention_kernel(const __gr
         __syncthreads();
         const int live_rows = min(kRows, p.rows - tile * kRows);
         // The CTAs that have a stretch of this job; a CTA's first stretch and its last one have places of their own.
-        const long long cta0 = p.whole ? 0 : job_at / share, cta1 = p.whole ? 0 : (job_at + quads - 1) / share;
+        const long long per = pieces ? 1 : share;                    // units of `at` a CTA
+        const long long cta0 = p.whole ? 0 : job_at / per, cta1 = p.whole ? 0 : (job_at + quads - 1) / per;
         const int used = (int)(cta1 - cta0) + 1;
         float* mypart = p.part + ((long long)blockIdx.x * 2 + (at != first)) * kPart;
         if (threadIdx.x < kRows) {
@@ -378,7 +401,7 @@ __global__ void __launch_bounds__(kWarps * 32) cache_attention_kernel(const __gr
             if (last) {
                 // part n is the first stretch of its CTA, but for a job that begins in the middle of a CTA's share
                 const float* parts = p.part + cta0 * 2 * kPart;
-                const int shift = job_at > cta0 * share ? kPart : 0;
+                const int shift = job_at > cta0 * per ? kPart : 0;
                 // All the maxima and sums, and as many parts as shared memory takes, come in one go; a thread copies what it
                 // will add up itself.
                 float* ml = reinterpret_cast<float*>(smem);    // [part]{ [8] maxima, then weights; [8] sums }
@@ -509,8 +532,11 @@ TensorData kv_cache_attention(KvCache& c, const TensorData& q_in, float scale, c
     out.buf = dev.alloc((size_t)std::max<int64_t>(out.layout.numel(), 1) * dtype_size(c.dtype), false);
     if (out.layout.numel() == 0) return out;
     for (const BufferRef& b : {c.codes, c.scales, c.tail, c.lens}) dev.note_recorded_buffer(b);
-    if (counts) kv_cache_set_counts(c, counts, t, "attention");
+    if (counts && dev.recording()) fail(WGF_ERR_UNSUPPORTED, "counts of an attention are fixed numbers: a recording takes none");
     AttParams p{};
+    p.use_counts = !counts ? 0 : c.batch <= kGiven ? 2 : 1;
+    if (p.use_counts == 1) kv_cache_set_counts(c, counts, t, "attention");
+    if (p.use_counts == 2) std::copy(counts, counts + c.batch, p.given);
     p.codes = (const uint8_t*)c.codes->ptr;
     p.scales = (const float*)c.scales->ptr;
     p.lens = (const int*)c.lens->ptr;
@@ -526,7 +552,6 @@ TensorData kv_cache_attention(KvCache& c, const TensorData& q_in, float scale, c
     p.q_heads = (int)s[1];
     p.group = (int)group;
     p.t = (int)t;
-    p.use_counts = counts != nullptr;
     p.rows = (int)(group * t);
     p.tiles = (p.rows + kRows - 1) / kRows;
     p.scale_log2 = scale * 1.4426950408889634f;

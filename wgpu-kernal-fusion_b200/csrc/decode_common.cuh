@@ -74,9 +74,33 @@ __device__ __forceinline__ unsigned abs_bits(float x) { return __float_as_uint(x
 // ---- one head: y = x / sqrt(mean(x^2) + eps) * w, then rotated by the position's angle -------------------
 // A group of `lanes` (a power of two, at most 32, neighbours in a warp) holds a row: lane l has the chunks
 // l, l + lanes, ... of VEC values of the first half, and the same chunks of the second half, which are the
-// partners of the rotation.  Everything is f32; the caller rounds once.
+// partners of the rotation.  A row stays as it was loaded until it is used.  Everything is f32 and rounded once.
+//
+// What a position does to a head: with w the weight,
+//   out_lo = (x_lo (w_lo cos) - x_hi (w_hi sin)) r,  out_hi = (x_hi (w_hi cos) + x_lo (w_lo sin)) r,
+// so weight and angle are multiplied once for all heads of a token.
+template <typename T, int VEC, int NCH> struct Turn {
+    float lc[NCH][VEC], ls[NCH][VEC], hc[NCH][VEC], hs[NCH][VEC];
+    __device__ __forceinline__ void load(const T* w, const T* cos, const T* sin, int half, int lane, int lanes) {
+        typedef Pack<T, VEC> V;
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) {
+            const int j = (lane + c * lanes) * VEC, at = j < half ? j : 0;
+            const V a = *reinterpret_cast<const V*>(w + at), b = *reinterpret_cast<const V*>(w + half + at);
+            const V cs = *reinterpret_cast<const V*>(cos + at), sn = *reinterpret_cast<const V*>(sin + at);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float lo = to_f<T>(a.v[e]), hi = to_f<T>(b.v[e]), x = to_f<T>(cs.v[e]), y = to_f<T>(sn.v[e]);
+                lc[c][e] = lo * x;
+                ls[c][e] = lo * y;
+                hc[c][e] = hi * x;
+                hs[c][e] = hi * y;
+            }
+        }
+    }
+};
 template <typename T, int VEC, int NCH> struct HeadRow {
-    float lo[NCH][VEC], hi[NCH][VEC];
+    Pack<T, VEC> lo[NCH], hi[NCH];
 
     __device__ __forceinline__ void load(const T* row, int half, int lane, int lanes) {
         typedef Pack<T, VEC> V;
@@ -84,15 +108,11 @@ template <typename T, int VEC, int NCH> struct HeadRow {
         for (int c = 0; c < NCH; ++c) {
             const int j = (lane + c * lanes) * VEC;
             if (j < half) {
-                const V a = *reinterpret_cast<const V*>(row + j), b = *reinterpret_cast<const V*>(row + half + j);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    lo[c][e] = to_f<T>(a.v[e]);
-                    hi[c][e] = to_f<T>(b.v[e]);
-                }
+                lo[c] = *reinterpret_cast<const V*>(row + j);
+                hi[c] = *reinterpret_cast<const V*>(row + half + j);
             } else {
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) lo[c][e] = hi[c][e] = 0.f;
+                for (int e = 0; e < VEC; ++e) lo[c].v[e] = hi[c].v[e] = from_f<T>(0.f);
             }
         }
     }
@@ -102,19 +122,26 @@ template <typename T, int VEC, int NCH> struct HeadRow {
 #pragma unroll
         for (int c = 0; c < NCH; ++c)
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) s += lo[c][e] * lo[c][e] + hi[c][e] * hi[c][e];
+            for (int e = 0; e < VEC; ++e) {
+                const float a = to_f<T>(lo[c].v[e]), b = to_f<T>(hi[c].v[e]);
+                s += a * a;
+                s += b * b;
+            }
         for (int m = lanes >> 1; m >= 1; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
         return 1.0f / sqrtf(s / (float)(2 * half) + eps);
     }
-    __device__ __forceinline__ void norm_rotate(const HeadRow& w, const float (&cs)[NCH][VEC], const float (&sn)[NCH][VEC], float r) {
+    // The normed and rotated row, rounded
+    __device__ __forceinline__ HeadRow turned(const Turn<T, VEC, NCH>& t, float r) const {
+        HeadRow y;
 #pragma unroll
         for (int c = 0; c < NCH; ++c)
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                const float a = lo[c][e] * r * w.lo[c][e], b = hi[c][e] * r * w.hi[c][e];
-                lo[c][e] = a * cs[c][e] - b * sn[c][e];
-                hi[c][e] = b * cs[c][e] + a * sn[c][e];
+                const float a = to_f<T>(lo[c].v[e]), b = to_f<T>(hi[c].v[e]);
+                y.lo[c].v[e] = from_f<T>((a * t.lc[c][e] - b * t.hs[c][e]) * r);
+                y.hi[c].v[e] = from_f<T>((b * t.hc[c][e] + a * t.ls[c][e]) * r);
             }
+        return y;
     }
     __device__ __forceinline__ void store(T* row, int half, int lane, int lanes) const {
         typedef Pack<T, VEC> V;
@@ -122,33 +149,11 @@ template <typename T, int VEC, int NCH> struct HeadRow {
         for (int c = 0; c < NCH; ++c) {
             const int j = (lane + c * lanes) * VEC;
             if (j >= half) continue;
-            V a, b;
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                a.v[e] = from_f<T>(lo[c][e]);
-                b.v[e] = from_f<T>(hi[c][e]);
-            }
-            *reinterpret_cast<V*>(row + j) = a;
-            *reinterpret_cast<V*>(row + half + j) = b;
+            *reinterpret_cast<V*>(row + j) = lo[c];
+            *reinterpret_cast<V*>(row + half + j) = hi[c];
         }
     }
 };
-template <typename T, int VEC, int NCH>
-__device__ __forceinline__ void load_half(const T* p, int half, int lane, int lanes, float (&v)[NCH][VEC]) {
-    typedef Pack<T, VEC> V;
-#pragma unroll
-    for (int c = 0; c < NCH; ++c) {
-        const int j = (lane + c * lanes) * VEC;
-        if (j < half) {
-            const V a = *reinterpret_cast<const V*>(p + j);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) v[c][e] = to_f<T>(a.v[e]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) v[c][e] = 0.f;
-        }
-    }
-}
 
 }  // namespace decode
 }  // namespace wgf

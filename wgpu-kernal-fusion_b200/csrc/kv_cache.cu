@@ -30,6 +30,8 @@ namespace {
 
 constexpr int kBlock = KvCache::kBlock;
 constexpr int kThreads = 256;
+constexpr int kGiven = 256;
+constexpr int kRecode = 1 << 30;
 
 struct CacheView {
     uint8_t* codes;
@@ -53,7 +55,7 @@ struct AppendParams {
     const void *k, *v;                     // [batch, heads, t, dim]
     long long kb, kh, ks, vb, vh, vs;      // strides of batch, head, token
     int t;                                 // new tokens a sequence; -1: none, sequences with a count are coded anew
-    int use_counts;
+    int use_counts;                        // 1: in the second half of the cache's lens, 2: in `given`
     int blocks_touched;                    // of one sequence, at most
     // keys behind norm and rotation, and the queries with them
     const void *wk, *wq, *cos, *sin, *q;
@@ -63,45 +65,100 @@ struct AppendParams {
     unsigned kv_ctas;                      // CTAs behind these do rows of q
     float eps;
     unsigned* ticket;
+    // Small batches' numbers by value, so that they cost no launch of their own: counts, or (t < 0) the new lengths, with
+    // kRecode where the open block's codes have to be made anew.
+    int given[kGiven];
 };
 
 __device__ __forceinline__ int key_token(int nt, int g) { return (g >> 1) * 16 + (nt >> 1) * 4 + (nt & 1) * 2 + (g & 1); }
 
-// Gathers block `blk` into tile[64][stride] (zero where it has no token) and returns this thread's largest
-// |x| as an ordered integer.  Tokens before `len` come from the tail, those up to `end` from the call.
-// With `keep`, new tokens go to the tail as well.
-template <typename T, int VEC, int NCH, bool NORM>
-__device__ unsigned gather(const AppendParams& p, T* tile, int stride, int b, int h, int blk, int kv, int len, int end, bool keep) {
-    const CacheView& c = p.c;
+// The block's tokens in shared memory: rows of dim_pad values in 16-byte pieces, the pieces of a row exchanged so that the
+// lanes of neither reading below, of eight tokens' pieces or of four groups of 16 tokens, meet in a bank.
+template <typename T, int DP> __device__ __forceinline__ int tile_at(int row, int j) {
+    constexpr int PIECE = 16 / (int)sizeof(T);
+    const int turn = sizeof(T) == 2 ? ((row >> 4) & 3) * 2 | (row & 1) : ((row >> 4) & 1) * 4 | (row & 1);
+    return row * DP + (j ^ (turn * PIECE));
+}
+
+// The largest |x|: two 16-bit ones side by side, or the bits of an f32.  As an ordered integer NaN is above infinity is above
+// every number; the maximum of pairs keeps a NaN.
+template <typename T> struct Largest {
     unsigned top = 0;
+    template <int VEC> __device__ __forceinline__ void take(const Pack<T, VEC>& x) {
+        if constexpr (sizeof(T) == 2 && VEC % 2 == 0) {
+            typedef typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type T2;
+            const T2* w = reinterpret_cast<const T2*>(&x);
+            T2 t = *reinterpret_cast<const T2*>(&top);
+#pragma unroll
+            for (int i = 0; i < VEC / 2; ++i) t = __hmax2_nan(t, __habs2(w[i]));
+            top = *reinterpret_cast<const unsigned*>(&t);
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                if constexpr (sizeof(T) == 2) top = max(top, *reinterpret_cast<const unsigned short*>(&x.v[e]) & 0x7fffu);
+                else top = max(top, abs_bits(x.v[e]));
+            }
+        }
+    }
+    // as the bits of an f32
+    __device__ __forceinline__ unsigned bits() const {
+        if constexpr (sizeof(T) == 2) {
+            const unsigned short h = (unsigned short)max(top & 0xffffu, top >> 16);
+            return abs_bits(to_f<T>(*reinterpret_cast<const T*>(&h)));
+        } else {
+            return top;
+        }
+    }
+};
+
+// Gathers block `blk` into the tile (zero where it has no token) and returns this thread's largest |x| as the bits of an f32.
+// Tokens before `len` come from the tail, those up to `end` from the call.  With `keep`, new tokens go to the tail as well.
+template <typename T, int DP, int VEC, int NCH, bool NORM>
+__device__ unsigned gather(const AppendParams& p, T* tile, int b, int h, int blk, int kv, int len, int end, bool keep) {
+    const CacheView& c = p.c;
+    Largest<T> top;
     const int first = blk * kBlock;
     const T* src = kv ? (const T*)p.v + b * p.vb + h * p.vh : (const T*)p.k + b * p.kb + h * p.kh;
     const long long step = kv ? p.vs : p.ks;
     T* tail = c.tail_of<T>(b, h, blk, kv);
     typedef Pack<T, VEC> V;
-    const int per_row = c.dim_pad / VEC;
     const bool turned = NORM && kv == 0;
-    for (int i = threadIdx.x; i < kBlock * per_row; i += kThreads) {
-        const int row = i / per_row, j = (i - row * per_row) * VEC, pos = first + row;
-        V x;
+    // a thread's pieces, one row and column behind the other; four loads at a time
+    constexpr int per_row = DP / VEC, row_step = kThreads / per_row, j_step = (kThreads - row_step * per_row) * VEC;
+    int row = threadIdx.x / per_row, j = (threadIdx.x - row * per_row) * VEC;
+    while (row < kBlock) {
+        V x[4];
+        int rows[4], js[4];
+        bool mine[4];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) x.v[e] = from_f<T>(0.f);
-        if (j < c.dim && pos < end) {
-            if (pos < len) x = *reinterpret_cast<const V*>(tail + (long long)row * c.dim + j);
-            else if (!turned) {
-                x = *reinterpret_cast<const V*>(src + (long long)(pos - len) * step + j);
-                if (keep) *reinterpret_cast<V*>(tail + (long long)row * c.dim + j) = x;
-            } else continue;                               // written below
+        for (int i = 0; i < 4; ++i) {
+            rows[i] = row;
+            js[i] = j;
+            const int pos = first + row;
+            mine[i] = row < kBlock && !(turned && j < c.dim && pos >= len && pos < end);      // those are written below
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) x[i].v[e] = from_f<T>(0.f);
+            if (mine[i] && j < c.dim && pos < end)
+                x[i] = *reinterpret_cast<const V*>(pos < len ? tail + (long long)row * c.dim + j : src + (long long)(pos - len) * step + j);
+            row += row_step;
+            j += j_step;
+            if (j_step && j >= DP) {
+                j -= DP;
+                ++row;
+            }
         }
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) top = max(top, abs_bits(to_f<T>(x.v[e])));
-        *reinterpret_cast<V*>(tile + row * stride + j) = x;
+        for (int i = 0; i < 4; ++i) {
+            if (!mine[i]) continue;
+            top.take(x[i]);
+            *reinterpret_cast<V*>(tile + tile_at<T, DP>(rows[i], js[i])) = x[i];
+            const int pos = first + rows[i];
+            if (keep && js[i] < c.dim && pos >= len && pos < end) *reinterpret_cast<V*>(tail + (long long)rows[i] * c.dim + js[i]) = x[i];
+        }
     }
     if (turned) {
         typedef HeadRow<T, VEC, NCH> Row;
         const int half = c.dim / 2, lane = threadIdx.x & (p.lanes - 1), groups = kThreads / p.lanes;
-        Row w;
-        w.load((const T*)p.wk, half, lane, p.lanes);
         const int begin = max(len, first), stop = min(end, first + kBlock);
         for (int base = begin; base < stop; base += groups) {      // all lanes of a warp stay together for the shuffles
             const int pos = base + threadIdx.x / p.lanes;
@@ -109,34 +166,52 @@ __device__ unsigned gather(const AppendParams& p, T* tile, int stride, int b, in
             const int at = live ? pos : begin;
             Row r;
             r.load(src + (long long)(at - len) * step, half, lane, p.lanes);
-            float cs[NCH][VEC], sn[NCH][VEC];
+            Turn<T, VEC, NCH> turn;
             const long long angle = min(at, p.table_rows - 1);
-            load_half<T, VEC, NCH>((const T*)p.cos + angle * p.cs_c, half, lane, p.lanes, cs);
-            load_half<T, VEC, NCH>((const T*)p.sin + angle * p.cs_s, half, lane, p.lanes, sn);
-            r.norm_rotate(w, cs, sn, r.inverse_rms(half, p.lanes, p.eps));
+            turn.load((const T*)p.wk, (const T*)p.cos + angle * p.cs_c, (const T*)p.sin + angle * p.cs_s, half, lane, p.lanes);
+            r = r.turned(turn, r.inverse_rms(half, p.lanes, p.eps));
             if (!live) continue;
 #pragma unroll
-            for (int n = 0; n < NCH; ++n)
-#pragma unroll
-                for (int e = 0; e < VEC; ++e)
-                    // the values that the operators one by one would hand over: rounded to the type
-                    top = max(top, max(abs_bits(to_f<T>(from_f<T>(r.lo[n][e]))), abs_bits(to_f<T>(from_f<T>(r.hi[n][e])))));
-            r.store(tile + (pos - first) * stride, half, lane, p.lanes);
+            for (int n = 0; n < NCH; ++n) {
+                const int j = (lane + n * p.lanes) * VEC;
+                if (j >= half) continue;
+                // the values that the operators one by one would hand over: rounded to the type
+                top.take(r.lo[n]);
+                top.take(r.hi[n]);
+                *reinterpret_cast<V*>(tile + tile_at<T, DP>(pos - first, j)) = r.lo[n];
+                *reinterpret_cast<V*>(tile + tile_at<T, DP>(pos - first, half + j)) = r.hi[n];
+            }
             if (keep) r.store(tail + (long long)(pos - first) * c.dim, half, lane, p.lanes);
         }
     }
-    return top;
+    return top.bits();
 }
 
-template <typename T>
-__device__ __forceinline__ unsigned code4(const T* x, int step, float k, float den, float inv) {
-    unsigned w = 0;
+__device__ __noinline__ unsigned four_exact(float x0, float x1, float x2, float x3, float num, float den, float inv) {
+    return (unsigned)(exact_code(x0, num, den, inv) + 128) | (unsigned)(exact_code(x1, num, den, inv) + 128) << 8 |
+           (unsigned)(exact_code(x2, num, den, inv) + 128) << 16 | (unsigned)(exact_code(x3, num, den, inv) + 128) << 24;
+}
+// Four values' codes + 128 as bytes.  x k is off by less than 2^-16, so the nearest whole number is the code unless the product is
+// that near to a border; `border` then tells, and the four are done over with exact_code.  Adding 1.5 * 2^23 + 128 leaves the
+// whole number in the low bits.
+struct Coder {
+    float k;            // 127 / max|x|
+    float num, den, inv;
+    static __device__ __forceinline__ float magic() { return 12582912.f + 128.f; }
+    __device__ __forceinline__ unsigned four(const float (&x)[4]) const {
+        float m[4], off = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w |= (unsigned)(exact_code(to_f<T>(x[i * step]), k, den, inv) + 128) << (8 * i);
-    return w;
-}
+        for (int i = 0; i < 4; ++i) {
+            m[i] = __fmaf_rn(x[i], k, magic());
+            off = fmaxf(off, fabsf(__fmaf_rn(x[i], k, -(m[i] - magic()))));
+        }
+        if (off > 0.5f - 0x1p-15f) return four_exact(x[0], x[1], x[2], x[3], num, den, inv);
+        const unsigned a = __byte_perm(__float_as_uint(m[0]), __float_as_uint(m[1]), 0x0040), b = __byte_perm(__float_as_uint(m[2]), __float_as_uint(m[3]), 0x0040);
+        return __byte_perm(a, b, 0x5410);
+    }
+};
 
-template <typename T, int VEC, int NCH, bool NORM>
+template <typename T, int DP, int VEC, int NCH, bool NORM>
 __global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_constant__ AppendParams p) {
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ unsigned warp_top[kThreads / 32];
@@ -149,19 +224,19 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_consta
         const int nb = i % p.blocks_touched;
         i /= p.blocks_touched;
         const int h = i % c.heads, b = i / c.heads;
-        const int len = c.lens[b];
-        const int asked = p.use_counts ? c.lens[c.batch + b] : p.t;
+        const int len = p.t < 0 && p.use_counts == 2 ? p.given[b] & (kRecode - 1) : c.lens[b];
+        const int asked = p.use_counts == 2 ? (p.t < 0 ? p.given[b] >> 30 : p.given[b]) : p.use_counts ? c.lens[c.batch + b] : p.t;
+        if (p.t < 0 && p.use_counts == 2 && nb + h + kv == 0 && threadIdx.x == 0) c.lens[b] = len;
         const int fresh = p.t < 0 ? 0 : min(asked, c.capacity - len);
         const int end = len + fresh, blk = len / kBlock + nb;
         T* tile = (T*)smem;
-        const int stride = c.dim_pad + 16 / (int)sizeof(T);        // rows 16 bytes apart in the banks
         if (p.t < 0 ? (asked > 0 && nb == 0 && len % kBlock != 0) : (fresh > 0 && blk * kBlock < end)) {
             // the two blocks that the tail keeps: the open one and the one before it
             const int open = end / kBlock, first_blk = len / kBlock;
             // a block of the same parity as the first one would overwrite what the first one's CTA reads: that CTA
             // writes it, after it has read
             const bool keep = blk >= open - 1 && (blk == first_blk || ((blk ^ first_blk) & 1));
-            unsigned top = gather<T, VEC, NCH, NORM>(p, tile, stride, b, h, blk, kv, len, end, keep && p.t > 0);
+            unsigned top = gather<T, DP, VEC, NCH, NORM>(p, tile, b, h, blk, kv, len, end, keep && p.t > 0);
             top = __reduce_max_sync(0xffffffffu, top);
             if ((threadIdx.x & 31) == 0) warp_top[threadIdx.x >> 5] = top;
             __syncthreads();
@@ -172,29 +247,50 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_consta
             const float amax = fmaxf(__uint_as_float(finite ? top : 0u), 0x1p-100f);
             // far up, 127 x would leave the range: both sides of the quotient come down by the same power of two
             const float down = amax > 0x1p100f ? 0x1p-32f : 1.f;
-            const float k = finite ? 127.f * down : 0.f, den = amax * down, inv = 1.f / den;
-            uint8_t* out = c.block(b, h, blk, kv);
+            Coder code;
+            code.k = finite ? 127.f / amax : 0.f;
+            code.num = finite ? 127.f * down : 0.f;
+            code.den = amax * down;
+            code.inv = 1.f / code.den;
+            uint4* out = reinterpret_cast<uint4*>(c.block(b, h, blk, kv));
+            const uint4 none = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
             if (kv == 0) {
-                for (int i = threadIdx.x; i < kBlock * (c.dim_pad / 16); i += kThreads) {
-                    const int lane = i & 31, j = (i >> 5) % (c.dim_pad / 64), nt = (i >> 5) / (c.dim_pad / 64);
-                    const T* x = tile + key_token(nt, lane >> 2) * stride + j * 64 + (lane & 3) * 16;
-                    uint4 w;
-                    w.x = code4<T>(x, 1, k, den, inv);
-                    w.y = code4<T>(x + 4, 1, k, den, inv);
-                    w.z = code4<T>(x + 8, 1, k, den, inv);
-                    w.w = code4<T>(x + 12, 1, k, den, inv);
-                    reinterpret_cast<uint4*>(out)[i] = finite ? w : make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+                // 16 dims of a token
+                for (int i = threadIdx.x; i < kBlock * (DP / 16); i += kThreads) {
+                    const int lane = i & 31, j = (i >> 5) % (DP / 64), nt = (i >> 5) / (DP / 64);
+                    const int row = key_token(nt, lane >> 2), at = j * 64 + (lane & 3) * 16;
+                    unsigned w[4];
+#pragma unroll
+                    for (int q = 0; q < 16; q += 16 / (int)sizeof(T)) {
+                        const Pack<T, 16 / sizeof(T)> x = *reinterpret_cast<const Pack<T, 16 / sizeof(T)>*>(tile + tile_at<T, DP>(row, at + q));
+#pragma unroll
+                        for (int e = 0; e < 16 / (int)sizeof(T); e += 4) {
+                            const float v[4] = {to_f<T>(x.v[e]), to_f<T>(x.v[e + 1]), to_f<T>(x.v[e + 2]), to_f<T>(x.v[e + 3])};
+                            w[(q + e) / 4] = code.four(v);
+                        }
+                    }
+                    out[i] = finite ? make_uint4(w[0], w[1], w[2], w[3]) : none;
                 }
             } else {
-                for (int i = threadIdx.x; i < kBlock * (c.dim_pad / 16); i += kThreads) {
-                    const int lane = i & 31, nd = i >> 5;
-                    const T* x = tile + (lane & 3) * 16 * stride + nd * 8 + (lane >> 2);
-                    uint4 w;
-                    w.x = code4<T>(x, stride, k, den, inv);
-                    w.y = code4<T>(x + 4 * stride, stride, k, den, inv);
-                    w.z = code4<T>(x + 8 * stride, stride, k, den, inv);
-                    w.w = code4<T>(x + 12 * stride, stride, k, den, inv);
-                    reinterpret_cast<uint4*>(out)[i] = finite ? w : make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+                // 16 tokens of two dims side by side
+                for (int i = threadIdx.x; i < kBlock * (DP / 32); i += kThreads) {
+                    const int c4 = i & 3, d = (i >> 2) * 2;
+                    unsigned w[2][4];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        float v[2][4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const Pack<T, 2> x = *reinterpret_cast<const Pack<T, 2>*>(tile + tile_at<T, DP>(c4 * 16 + q * 4 + e, d));
+                            v[0][e] = to_f<T>(x.v[0]);
+                            v[1][e] = to_f<T>(x.v[1]);
+                        }
+                        w[0][q] = code.four(v[0]);
+                        w[1][q] = code.four(v[1]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        out[(d >> 3) * 32 + ((d & 7) + e) * 4 + c4] = finite ? make_uint4(w[e][0], w[e][1], w[e][2], w[e][3]) : none;
                 }
             }
             if (threadIdx.x == 0) *c.scale(b, h, blk, kv) = finite ? amax / 127.f : __uint_as_float(0x7fc00000u);
@@ -202,7 +298,7 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_consta
                 for (int x = max(open - 1, first_blk + 1); x <= open; ++x)
                     if (!((x ^ first_blk) & 1) && x * kBlock < end) {
                         __syncthreads();
-                        gather<T, VEC, NCH, NORM>(p, tile, stride, b, h, x, kv, len, end, true);
+                        gather<T, DP, VEC, NCH, NORM>(p, tile, b, h, x, kv, len, end, true);
                     }
             }
         }
@@ -215,22 +311,19 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_consta
         const int s = (int)(at % p.t);
         const long long o = at / p.t;
         const int h = (int)(o % p.q_heads), b = (int)(o / p.q_heads);
-        const int len = c.lens[b], asked = p.use_counts ? c.lens[c.batch + b] : p.t;
-        Row r, w;
+        const int len = c.lens[b], asked = p.use_counts == 2 ? p.given[b] : p.use_counts ? c.lens[c.batch + b] : p.t;
+        Row r;
         r.load((const T*)p.q + b * p.qb + h * p.qh + s * p.qs, half, lane, p.q_lanes);
-        w.load((const T*)p.wq, half, lane, p.q_lanes);
-        float cs[NCH][VEC], sn[NCH][VEC];
+        Turn<T, VEC, NCH> turn;
         const long long angle = min(len + s, p.table_rows - 1);
-        load_half<T, VEC, NCH>((const T*)p.cos + angle * p.cs_c, half, lane, p.q_lanes, cs);
-        load_half<T, VEC, NCH>((const T*)p.sin + angle * p.cs_s, half, lane, p.q_lanes, sn);
-        const float inv = r.inverse_rms(half, p.q_lanes, p.eps);
+        turn.load((const T*)p.wq, (const T*)p.cos + angle * p.cs_c, (const T*)p.sin + angle * p.cs_s, half, lane, p.q_lanes);
+        r = r.turned(turn, r.inverse_rms(half, p.q_lanes, p.eps));
         if (row < rows) {
-            r.norm_rotate(w, cs, sn, inv);
             if (s >= asked) {      // a padding row: zeros, whatever it held
 #pragma unroll
                 for (int n = 0; n < NCH; ++n)
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) r.lo[n][e] = r.hi[n][e] = 0.f;
+                    for (int e = 0; e < VEC; ++e) r.lo[n].v[e] = r.hi[n].v[e] = from_f<T>(0.f);
             }
             r.store((T*)p.q_out + row * c.dim, half, lane, p.q_lanes);
         }
@@ -242,7 +335,7 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_consta
     __syncthreads();
     if (last) {
         for (int b = threadIdx.x; b < c.batch; b += kThreads) {
-            const int len = c.lens[b], asked = p.use_counts ? c.lens[c.batch + b] : p.t;
+            const int len = c.lens[b], asked = p.use_counts == 2 ? p.given[b] : p.use_counts ? c.lens[c.batch + b] : p.t;
             c.lens[b] = len + min(asked, c.capacity - len);
         }
         if (threadIdx.x == 0) *p.ticket = 0;
@@ -259,10 +352,12 @@ __global__ void kv_set_kernel(const __grid_constant__ SetParams p) {
     for (int i = threadIdx.x; i < p.n; i += blockDim.x) p.to[i] = p.v[i];
 }
 
-template <typename T>
+// The number that a byte stands for: it is put under the exponent of 2^23, and 2^23 + 128 is taken off
+__device__ __forceinline__ float byte_code(unsigned w, int i) { return __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 | i)) - 8388736.f; }
+
+template <typename T, int DP>
 __global__ void __launch_bounds__(kThreads) kv_read_kernel(const __grid_constant__ CacheView c, T* __restrict__ k_out,
                                                            T* __restrict__ v_out, int longest, int out_blocks) {
-    extern __shared__ __align__(16) unsigned char smem[];
     const int kv = blockIdx.x & 1;
     unsigned i = blockIdx.x >> 1;
     const int blk = i % out_blocks;
@@ -270,35 +365,50 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const __grid_constant
     const int h = i % c.heads, b = i / c.heads;
     const int rows = min(kBlock, longest - blk * kBlock), have = min(max(c.lens[b] - blk * kBlock, 0), rows);
     T* out = (kv ? v_out : k_out) + (((long long)b * c.heads + h) * longest + blk * kBlock) * (long long)c.dim;
-    // the codes as [token][dim] in shared memory, then rows of values
-    const int stride = c.dim_pad + 16;
-    if (have > 0) {
-        const uint4* in = reinterpret_cast<const uint4*>(c.block(b, h, blk, kv));
-        for (int n = threadIdx.x; n < kBlock * (c.dim_pad / 16); n += kThreads) {
-            const uint4 w = in[n];
-            const int lane = n & 31;
-            if (kv == 0) {
-                const int j = (n >> 5) % (c.dim_pad / 64), nt = (n >> 5) / (c.dim_pad / 64);
-                *reinterpret_cast<uint4*>(smem + key_token(nt, lane >> 2) * stride + j * 64 + (lane & 3) * 16) = w;
-            } else {
-                const unsigned v[4] = {w.x, w.y, w.z, w.w};
-                uint8_t* x = smem + (lane & 3) * 16 * stride + (n >> 5) * 8 + (lane >> 2);
+    const float scale = have > 0 ? *c.scale(b, h, blk, kv) : 0.f;
+    const uint4* in = reinterpret_cast<const uint4*>(c.block(b, h, blk, kv));
+    if (kv == 0) {
+        // 16 dims of a token are 16 values in a row
+        for (int n = threadIdx.x; n < kBlock * (DP / 16); n += kThreads) {
+            const int lane = n & 31, j = (n >> 5) % (DP / 64), nt = (n >> 5) / (DP / 64);
+            const int row = key_token(nt, lane >> 2), d = j * 64 + (lane & 3) * 16;
+            if (row >= rows || d >= c.dim) continue;
+            const uint4 u = row < have ? in[n] : make_uint4(0, 0, 0, 0);
+            const unsigned w[4] = {u.x, u.y, u.z, u.w};
+            constexpr int W = 16 / (int)sizeof(T) < 8 ? 16 / (int)sizeof(T) : 8;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) x[e * stride] = (uint8_t)(v[e >> 2] >> (8 * (e & 3)));
+            for (int q = 0; q < 16; q += W) {
+                if (d + q >= c.dim) break;                     // head_dim is a multiple of 8
+                Pack<T, W> x;
+#pragma unroll
+                for (int e = 0; e < W; ++e) x.v[e] = from_f<T>(row < have ? byte_code(w[(q + e) >> 2], (q + e) & 3) * scale : 0.f);
+                *reinterpret_cast<Pack<T, W>*>(out + (long long)row * c.dim + d + q) = x;
             }
         }
-    }
-    __syncthreads();
-    const float scale = have > 0 ? *c.scale(b, h, blk, kv) : 0.f;
-    constexpr int W = 16 / (int)sizeof(T);
-    const int per_row = c.dim / W;       // head_dim is a multiple of 8
-    for (int n = threadIdx.x; n < rows * per_row; n += kThreads) {
-        const int row = n / per_row, j = (n - row * per_row) * W;
-        const Pack<uint8_t, W> u = *reinterpret_cast<const Pack<uint8_t, W>*>(smem + row * stride + j);
-        Pack<T, W> x;
+    } else {
+        // 16 tokens of four dims: their bytes are turned four by four
+        for (int n = threadIdx.x; n < DP; n += kThreads) {
+            const int c4 = n / (DP / 4), d = n % (DP / 4) * 4;
+            if (d >= c.dim || c4 * 16 >= rows) continue;
+            uint4 u[4];
 #pragma unroll
-        for (int e = 0; e < W; ++e) x.v[e] = from_f<T>(row < have ? (float)((int)u.v[e] - 128) * scale : 0.f);
-        *reinterpret_cast<Pack<T, W>*>(out + (long long)row * c.dim + j) = x;
+            for (int e = 0; e < 4; ++e) u[e] = c4 * 16 < have ? in[(d >> 3) * 32 + ((d & 7) + e) * 4 + c4] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                unsigned w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = q == 0 ? u[e].x : q == 1 ? u[e].y : q == 2 ? u[e].z : u[e].w;
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    const int row = c4 * 16 + q * 4 + t;
+                    if (row >= rows) break;
+                    Pack<T, 4> x;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x.v[e] = from_f<T>(row < have ? byte_code(w[e], t) * scale : 0.f);
+                    *reinterpret_cast<Pack<T, 4>*>(out + (long long)row * c.dim + d) = x;
+                }
+            }
+        }
     }
 }
 
@@ -360,28 +470,39 @@ void set_ints(Device& dev, int* to, const std::vector<int>& v, const char* what)
 }
 
 template <typename F> void allow_smem(Device& dev, F kernel, size_t bytes) {
-    if (bytes > 48 * 1024 && !dev.dry) WGF_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    // 48 KiB need no leave, what the kernels declare among them
+    if (bytes > 47 * 1024 && !dev.dry) WGF_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+}
+
+template <typename F> void for_pad(int64_t dim_pad, F&& f) {
+    switch (dim_pad) {
+        case 64: return f(std::integral_constant<int, 64>());
+        case 128: return f(std::integral_constant<int, 128>());
+        case 192: return f(std::integral_constant<int, 192>());
+        default: return f(std::integral_constant<int, 256>());
+    }
 }
 
 template <typename T, int VEC, int NCH>
 void launch_append(Device& dev, const AppendParams& p, unsigned q_ctas, bool norm, const char* what) {
-    const size_t smem = (size_t)kBlock * (p.c.dim_pad + 16 / sizeof(T)) * sizeof(T);
-    const unsigned grid = p.kv_ctas + q_ctas;
-    auto go = [&](auto kernel) {
-        allow_smem(dev, kernel, smem);
-        dev.begin_launch(what);
-        if (!dev.dry) kernel<<<grid, kThreads, smem, dev.stream>>>(p);
-        dev.end_launch();
-    };
-    if (norm) go(kv_append_kernel<T, VEC, NCH, true>);
-    else go(kv_append_kernel<T, VEC, NCH, false>);
+    for_pad(p.c.dim_pad, [&](auto pad) {
+        constexpr int DP = decltype(pad)::value;
+        const size_t smem = (size_t)kBlock * DP * sizeof(T);
+        auto go = [&](auto kernel) {
+            allow_smem(dev, kernel, smem);
+            dev.begin_launch(what);
+            if (!dev.dry) kernel<<<p.kv_ctas + q_ctas, kThreads, smem, dev.stream>>>(p);
+            dev.end_launch();
+        };
+        if (norm) go(kv_append_kernel<T, DP, VEC, NCH, true>);
+        else go(kv_append_kernel<T, DP, VEC, NCH, false>);
+    });
 }
 
 template <typename T>
 void dispatch_append(Device& dev, const AppendParams& p, const RowSpread& s, unsigned q_ctas, bool norm, const char* what) {
     constexpr int W = 16 / (int)sizeof(T);
     if (s.vec == W) launch_append<T, W, 1>(dev, p, q_ctas, norm, what);        // dim <= 256: one chunk a lane
-    else if (s.vec == 4) launch_append<T, 4, 1>(dev, p, q_ctas, norm, what);
     else launch_append<T, 1, 4>(dev, p, q_ctas, norm, what);
 }
 
@@ -483,7 +604,9 @@ TensorData append(KvCache& c, const TensorData& k_in, const TensorData& v_in, co
     }
     for (const TensorData* x : {&k, &v}) dev.wait_for(*x->buf);
     note(c);
-    if (counts) kv_cache_set_counts(c, counts, t, "append");
+    p.use_counts = !counts ? 0 : c.batch <= kGiven ? 2 : 1;
+    if (p.use_counts == 1) kv_cache_set_counts(c, counts, t, "append");
+    if (p.use_counts == 2) std::copy(counts, counts + c.batch, p.given);
     p.c = view_of(c);
     p.k = k.base_ptr();
     p.v = v.base_ptr();
@@ -494,7 +617,6 @@ TensorData append(KvCache& c, const TensorData& k_in, const TensorData& v_in, co
     p.vh = v.layout.strides[1];
     p.vs = v.layout.strides[2];
     p.t = (int)t;
-    p.use_counts = counts != nullptr;
     p.blocks_touched = (int)((t + kBlock - 2) / kBlock + 1);
     run_append(dev, c, p, s, q_ctas, q_in != nullptr, q_in ? "kv_append_qk" : "kv_append");
     if (dev.recording()) {
@@ -577,16 +699,20 @@ void kv_cache_truncate(KvCache& c, const int64_t* lengths) {
         recode = recode || touched[b];
     }
     dev.make_current();
-    set_ints(dev, (int*)c.lens->ptr, lens, "kv_truncate");
-    if (recode) {
-        set_ints(dev, (int*)c.lens->ptr + c.batch, touched, "kv_counts");
-        AppendParams p{};
-        p.c = view_of(c);
-        p.t = -1;
+    AppendParams p{};
+    p.c = view_of(c);
+    p.t = -1;
+    p.blocks_touched = 1;
+    const bool by_value = recode && c.batch <= kGiven;
+    if (by_value) {
+        p.use_counts = 2;
+        for (int64_t b = 0; b < c.batch; ++b) p.given[b] = lens[b] | (touched[b] ? kRecode : 0);
+    } else {
+        set_ints(dev, (int*)c.lens->ptr, lens, "kv_truncate");
+        if (recode) set_ints(dev, (int*)c.lens->ptr + c.batch, touched, "kv_counts");
         p.use_counts = 1;
-        p.blocks_touched = 1;
-        run_append(dev, c, p, head_spread(c.dtype, c.dim, {c.tail->ptr}, {}), 0, false, "kv_recode");
     }
+    if (recode) run_append(dev, c, p, head_spread(c.dtype, c.dim, {c.tail->ptr}, {}), 0, false, "kv_recode");
     for (int64_t b = 0; b < c.batch; ++b) {
         c.lengths[b] = lengths[b];
         c.held_from[b] = std::min(c.held_from[b], lengths[b] / kBlock);
@@ -615,15 +741,17 @@ void kv_cache_read(KvCache& c, TensorData& k, TensorData& v) {
     if (n == 0) return;
     const int64_t out_blocks = (n + kBlock - 1) / kBlock, ctas = 2 * c.batch * c.heads * out_blocks;
     WGF_CHECK(ctas < (1ll << 31), WGF_ERR_UNSUPPORTED, "read of more than 2^30 blocks in one call");
-    const size_t smem = (size_t)kBlock * (c.dim_pad + 16);
     auto go = [&](auto kernel, auto* ko, auto* vo) {
         dev.begin_launch("kv_read");
-        if (!dev.dry) kernel<<<(unsigned)ctas, kThreads, smem, dev.stream>>>(view_of(c), ko, vo, (int)n, (int)out_blocks);
+        if (!dev.dry) kernel<<<(unsigned)ctas, kThreads, 0, dev.stream>>>(view_of(c), ko, vo, (int)n, (int)out_blocks);
         dev.end_launch();
     };
-    if (c.dtype == DType::F32) go(kv_read_kernel<float>, (float*)k.buf->ptr, (float*)v.buf->ptr);
-    else if (c.dtype == DType::F16) go(kv_read_kernel<__half>, (__half*)k.buf->ptr, (__half*)v.buf->ptr);
-    else go(kv_read_kernel<__nv_bfloat16>, (__nv_bfloat16*)k.buf->ptr, (__nv_bfloat16*)v.buf->ptr);
+    for_pad(c.dim_pad, [&](auto pad) {
+        constexpr int DP = decltype(pad)::value;
+        if (c.dtype == DType::F32) go(kv_read_kernel<float, DP>, (float*)k.buf->ptr, (float*)v.buf->ptr);
+        else if (c.dtype == DType::F16) go(kv_read_kernel<__half, DP>, (__half*)k.buf->ptr, (__half*)v.buf->ptr);
+        else go(kv_read_kernel<__nv_bfloat16, DP>, (__nv_bfloat16*)k.buf->ptr, (__nv_bfloat16*)v.buf->ptr);
+    });
 }
 
 }  // namespace wgf
