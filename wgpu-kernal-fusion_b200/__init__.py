@@ -37,6 +37,9 @@ class WgfError(RuntimeError):
         self.status = STATUS.get(code, str(code))
 
 
+_Extents = C.c_int64 * MAX_RANK
+
+
 class TensorDesc(C.Structure):
     _fields_ = [("buf", C.c_void_p), ("dtype", C.c_uint32), ("rank", C.c_uint32), ("offset", C.c_int64),
                 ("shape", C.c_int64 * MAX_RANK), ("stride", C.c_int64 * MAX_RANK)]
@@ -48,6 +51,17 @@ class EwOp(C.Structure):
 
 _lib = None
 
+# Parameter types of the calls that a decode loop makes many times: plain numbers are then passed as they are, which costs
+# about half as much as wrapping each of them.
+_P, _U32, _I64, _F = C.c_void_p, C.c_uint32, C.c_int64, C.c_float
+_PROTOTYPES = {
+    "wgf_tensor_release": [_P], "wgf_tensor_info": [_P] * 4, "wgf_tensor_materialize": [_P], "wgf_tensor_desc_of": [_P, _P],
+    "wgf_tensor_transpose": [_P, _U32, _U32, _P], "wgf_buffer_release": [_P], "wgf_buffer_device_ptr": [_P, _P, _P],
+    "wgf_tensor_qk_norm_rope": [_P] * 6 + [_F, _I64, _P, _P], "wgf_tensor_matmul_q4": [_P, _P, _P],
+    "wgf_kv_cache_truncate": [_P, _P], "wgf_kv_cache_append": [_P] * 4, "wgf_kv_cache_append_qk": [_P] * 8 + [_F, _P, _P],
+    "wgf_kv_cache_attention": [_P, _P, _F, _P, _P], "wgf_kv_cache_read": [_P] * 3, "wgf_schedule_launch": [_P],
+}
+
 
 def lib():
     """Loads libwgf.so (built by build.py).  Fails loudly when it is missing."""
@@ -58,6 +72,8 @@ def lib():
         os.environ.setdefault("WGF_KERNEL_CACHE", os.path.join(HERE, "_jit_cache"))
         _lib = C.CDLL(LIB_PATH)
         _lib.wgf_last_error.restype = C.c_char_p
+        for name, types in _PROTOTYPES.items():
+            getattr(_lib, name).argtypes = types
     return _lib
 
 
@@ -166,8 +182,9 @@ class Tensor:
         self.h = handle
 
     def __del__(self):
-        if getattr(self, "h", None) and _lib is not None:
-            _lib.wgf_tensor_release(self.h)
+        h = self.h
+        if h and _lib is not None:
+            _lib.wgf_tensor_release(h)
             self.h = None
 
     # ---- construction / introspection -------------------------------------------------
@@ -187,9 +204,9 @@ class Tensor:
 
     def _info(self):
         dt, rk = C.c_uint32(), C.c_uint32()
-        shp = (C.c_int64 * MAX_RANK)()
-        check(lib().wgf_tensor_info(self.h, C.byref(dt), C.byref(rk), shp))
-        return dt.value, tuple(shp[i] for i in range(rk.value))
+        shp = _Extents()
+        check(_lib.wgf_tensor_info(self.h, C.byref(dt), C.byref(rk), shp))
+        return dt.value, tuple(shp[:rk.value])
 
     @property
     def shape(self):
@@ -289,7 +306,7 @@ class Tensor:
         return self._un(lib().wgf_tensor_slice, _i64([r[0] for r in ranges]), _i64([r[1] for r in ranges]))
 
     def transpose(self, a, b):
-        return self._un(lib().wgf_tensor_transpose, C.c_uint32(a), C.c_uint32(b))
+        return self._un(_lib.wgf_tensor_transpose, a, b)
 
     def broadcast(self, out_shape):
         return self._un(lib().wgf_tensor_broadcast, C.c_uint32(len(out_shape)), _i64(out_shape))
@@ -369,8 +386,7 @@ class Tensor:
         """Each head of self (queries) and k normed, scaled by its weight and rotated by its position, start on:
         one kernel for both (wgf_tensor_qk_norm_rope).  Returns (q, k)."""
         q_out, k_out = C.c_void_p(), C.c_void_p()
-        check(lib().wgf_tensor_qk_norm_rope(self.h, k.h, q_weight.h, k_weight.h, cos.h, sin.h, C.c_float(eps), C.c_int64(start),
-                                            C.byref(q_out), C.byref(k_out)))
+        check(_lib.wgf_tensor_qk_norm_rope(self.h, k.h, q_weight.h, k_weight.h, cos.h, sin.h, eps, start, C.byref(q_out), C.byref(k_out)))
         return Tensor(self.dev, q_out), Tensor(self.dev, k_out)
 
     def quantize_q4(self, group=128):
@@ -381,7 +397,7 @@ class Tensor:
 
     def mat_mul_q4(self, w):
         """self [.., k] times the transposed 4-bit weights: [.., n] (wgf_tensor_matmul_q4)."""
-        return self._un(lambda h, out: lib().wgf_tensor_matmul_q4(h, w.h, out))
+        return self._un(_lib.wgf_tensor_matmul_q4, w.h)
 
     def all_reduce(self, comm, op=OP_SUM):
         out = C.c_void_p()
@@ -390,7 +406,7 @@ class Tensor:
 
     # ---- materialisation ---------------------------------------------------------------
     def materialize(self):
-        check(lib().wgf_tensor_materialize(self.h))
+        check(_lib.wgf_tensor_materialize(self.h))
         return self
 
     @staticmethod
@@ -403,7 +419,7 @@ class Tensor:
 
     def desc(self):
         d = TensorDesc()
-        check(lib().wgf_tensor_desc_of(self.h, C.byref(d)))
+        check(_lib.wgf_tensor_desc_of(self.h, C.byref(d)))
         return d
 
     def as_slice(self):
@@ -510,7 +526,7 @@ class Schedule:
         return False
 
     def launch(self):
-        check(lib().wgf_schedule_launch(self.h))
+        check(_lib.wgf_schedule_launch(self.h))
 
     @property
     def kernel_count(self):
@@ -533,7 +549,8 @@ class KvCache:
     """8-bit key/value cache (wgf_kv_cache_*).  Calls run at once, in the order in which they are made."""
 
     def __init__(self, dev, batch, kv_heads, head_dim, capacity, dtype=F16):
-        self.dev, self.batch = dev, batch
+        self.dev, self.batch, self.head_dim = dev, batch, head_dim
+        self._array = C.c_int64 * batch if batch > 0 else None
         self.h = C.c_void_p()
         check(lib().wgf_kv_cache_create(dev.h, C.c_uint32(dtype), C.c_int64(batch), C.c_int64(kv_heads), C.c_int64(head_dim),
                                         C.c_int64(capacity), C.byref(self.h)))
@@ -548,41 +565,41 @@ class KvCache:
             return None
         if len(values) != self.batch:
             raise ValueError(f"{len(values)} numbers for {self.batch} sequences")
-        return _i64(values)
+        return self._array(*[int(v) for v in values])
 
     @property
     def lengths(self):
-        out = (C.c_int64 * self.batch)()
+        out = self._array()
         check(lib().wgf_kv_cache_lengths(self.h, out))
         return list(out)
 
     def truncate(self, lengths):
         """Takes tokens back: new lengths, none above the present ones (wgf_kv_cache_truncate)."""
-        check(lib().wgf_kv_cache_truncate(self.h, self._numbers(lengths)))
+        check(_lib.wgf_kv_cache_truncate(self.h, self._numbers(lengths)))
 
     def append(self, k, v, counts=None):
         """k, v [batch, kv_heads, tokens, head_dim]; counts: tokens that each sequence takes (default: all)."""
-        check(lib().wgf_kv_cache_append(self.h, k.h, v.h, self._numbers(counts)))
+        check(_lib.wgf_kv_cache_append(self.h, k.h, v.h, self._numbers(counts)))
 
     def append_qk(self, q, k, v, q_weight, k_weight, cos, sin, eps=1e-6, counts=None):
         """Norm and rotation of q and k at each sequence's own positions, and append, in one launch; returns q."""
         out = C.c_void_p()
-        check(lib().wgf_kv_cache_append_qk(self.h, q.h, k.h, v.h, q_weight.h, k_weight.h, cos.h, sin.h, C.c_float(eps),
-                                           self._numbers(counts), C.byref(out)))
+        check(_lib.wgf_kv_cache_append_qk(self.h, q.h, k.h, v.h, q_weight.h, k_weight.h, cos.h, sin.h, eps, self._numbers(counts),
+                                          C.byref(out)))
         return Tensor(self.dev, out)
 
     def attention(self, q, scale=None, counts=None):
         """softmax(scale q K^T) V for q [batch, heads, tokens, head_dim] at the sequences' last positions."""
         if scale is None:
-            scale = 1.0 / float(np.sqrt(q.shape[-1]))
+            scale = self.head_dim ** -0.5
         out = C.c_void_p()
-        check(lib().wgf_kv_cache_attention(self.h, q.h, C.c_float(scale), self._numbers(counts), C.byref(out)))
+        check(_lib.wgf_kv_cache_attention(self.h, q.h, scale, self._numbers(counts), C.byref(out)))
         return Tensor(self.dev, out)
 
     def read(self):
         """(k, v): the values that the codes stand for, [batch, kv_heads, longest length, head_dim]."""
         k, v = C.c_void_p(), C.c_void_p()
-        check(lib().wgf_kv_cache_read(self.h, C.byref(k), C.byref(v)))
+        check(_lib.wgf_kv_cache_read(self.h, C.byref(k), C.byref(v)))
         return Tensor(self.dev, k), Tensor(self.dev, v)
 
 

@@ -113,6 +113,10 @@ Layout ViewOp::apply(const Layout& in) const {
                     out.strides[i] = 0;
                 }
             break;
+        case Part:                      // of a dense tensor
+            out = Layout::contiguous(shape);
+            out.offset = in.offset + size;
+            break;
     }
     return out;
 }
@@ -402,11 +406,17 @@ std::pair<NodeRef, NodeRef> op_qk_norm_rope(const NodeRef& q, const NodeRef& k, 
               "qk_norm_rope cos / sin must be equal [positions, head_dim / 2]");
     WGF_CHECK(start >= 0 && start <= cos->shape[0] && S <= cos->shape[0] - start, WGF_ERR_SHAPE, "qk_norm_rope: positions past the end of cos / sin");
     for (const NodeRef& n : {k, wq, wk, cos, sin}) WGF_CHECK(n->dtype == q->dtype, WGF_ERR_DTYPE, "qk_norm_rope element types differ");
-    const int64_t nq = q->numel(), nk = k->numel(), at = qk_second_offset(nq);
+    const int64_t nk = k->numel(), at = qk_second_offset(q->numel());
     auto both = new_node(NodeKind::QkNormRope, q->dev, {at + nk}, q->dtype, {q, k, wq, wk, cos, sin});
     both->imm = eps;
     both->starts = {start, at};
-    return {op_reshape(view_slice(both, {0}, {nq}), q->shape), op_reshape(view_slice(both, {at}, {at + nk}), k->shape)};
+    ViewOp part;
+    part.kind = ViewOp::Part;
+    part.shape = q->shape;
+    NodeRef q_out = make_view(both, part);
+    part.shape = k->shape;
+    part.size = at;
+    return {q_out, make_view(both, part)};
 }
 
 NodeRef op_matmul_q4(const NodeRef& x, const std::shared_ptr<Q4Weight>& w) {

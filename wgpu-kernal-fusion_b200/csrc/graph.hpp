@@ -26,12 +26,12 @@ enum class NodeKind : uint8_t {
 };
 
 struct ViewOp {
-    enum Kind : uint8_t { Slice, Transpose, BroadcastAxis, Expand } kind = Slice;
+    enum Kind : uint8_t { Slice, Transpose, BroadcastAxis, Expand, Part } kind = Slice;
     std::vector<int64_t> starts, ends;  // Slice
     int a = 0, b = 0;                   // Transpose
     int axis = 0;                       // BroadcastAxis: position of the new stride-0 axis
     int64_t size = 0;                   //                and its extent
-    std::vector<int64_t> shape;         // Expand: target shape
+    std::vector<int64_t> shape;         // Expand: target shape; Part: a dense tensor of this shape from element `size` on
     Layout apply(const Layout& in) const;
 };
 
