@@ -373,18 +373,76 @@ def test_q4_product(kind, rows, n, k, group, wgf, dev):
 
 
 @pytest.mark.parametrize("kind", KINDS)
-@pytest.mark.parametrize("rows,n,k,group,written_out", [(700, 72, 64, 32, ["f32"]), (3001, 130, 70, 32, ["f32"]), (200, 40, 300, 128, []), (65, 300, 1100, 64, []),
-                                                        (600, 1500, 2100, 64, KINDS)])
-def test_q4_product_of_many_rows(kind, rows, n, k, group, written_out, wgf, dev):
-    """Rows in blocks, and weights that are written out for the matrix product, in padded rows where k is odd for it."""
+@pytest.mark.parametrize("rows,n,k,group,way", [(700, 72, 64, 32, {"f32": "q4_dequantize"}), (3001, 130, 70, 32, {"f32": "q4_dequantize"}), (200, 40, 300, 128, {}), (65, 300, 1100, 64, {}),
+                                                (600, 1500, 2100, 64, {"f32": "q4_dequantize", "f16": "q4_tc", "bf16": "q4_tc"}),
+                                                (2300, 3400, 260, 64, {"f32": "q4_dequantize"})])
+def test_q4_product_of_many_rows(kind, rows, n, k, group, way, wgf, dev):
+    """Rows in blocks, on the tensor cores, and weights that are written out for the matrix product, in padded rows where k is odd for it."""
     g = seeded(23, rows)
     w, x = draw(g, (n, k), kind, 0.02), draw(g, (rows, k), kind)
     c, s = ref.q4_quantize(w, group, kind)
     t = give(wgf, dev, w, kind).quantize_q4(group)
     dev.set_timing(True)
     out = give(wgf, dev, x, kind).mat_mul_q4(t)
-    close(take(out, kind), *ref.q4_product(x, ref.q4_values(c, s, group), kind, through=kind if kind in written_out else None))
-    assert ("q4_dequantize" in out.timing_labels()) == (kind in written_out)
+    # rounded on the way, but in blocks
+    close(take(out, kind), *ref.q4_product(x, ref.q4_values(c, s, group), kind, through=kind))
+    if kind in way:
+        assert way[kind] in out.timing_labels()
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("scale_kind", KINDS)
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("rows,n,k", [(300, 1100, 1100), (257, 1030, 1091), (320, 2200, 1985), (1000, 260, 1024), (72, 9000, 2112)])
+def test_q4_product_on_tensor_cores(kind, scale_kind, group, rows, n, k, wgf, dev):
+    """Last tiles, steps and groups that are not full; scales of the rows' own type and of others."""
+    g = seeded(29, rows + n + k + group)
+    w, x = draw(g, (n, k), scale_kind, 0.02), draw(g, (rows, k), kind)
+    c, s = ref.q4_quantize(w, group, scale_kind)
+    t = give(wgf, dev, w, scale_kind).quantize_q4(group)
+    dev.set_timing(True)
+    out = give(wgf, dev, x, kind).mat_mul_q4(t)
+    close(take(out, kind), *ref.q4_product(x, ref.q4_values(c, s, group), kind, through=kind))
+    assert "q4_tc" in out.timing_labels()
+
+
+def test_q4_product_on_tensor_cores_of_bad_values_and_views(wgf, dev):
+    g = seeded(29, 1)
+    rows, n, k = 300, 1100, 1091
+    w, x = draw(g, (n, k), "f16", 0.02), draw(g, (rows, k + 5), "f16")
+    w[7, 1090] = np.inf                     # the last group of one row has no scale
+    t = give(wgf, dev, w, "f16").quantize_q4(64)
+    x[3, 5], x[4, 6] = np.nan, np.inf
+    dev.set_timing(True)
+    whole = give(wgf, dev, x, "f16")
+    out = whole.slice([(0, rows), (5, k + 5)]).mat_mul_q4(t)
+    got = np.asarray(take(out, "f16"))
+    assert "q4_tc" in out.timing_labels()
+    assert np.isnan(got[:, 7]).all() and np.isnan(got[3]).all()
+    keep_rows, keep = [r for r in range(rows) if r not in (3, 4)], [c for c in range(n) if c != 7]
+    assert not np.isfinite(got[4][keep]).any()
+    w[7] = 0
+    c, s = ref.q4_quantize(w, 64, "f16")
+    want, bound = ref.q4_product(x[keep_rows][:, 5:], ref.q4_values(c, s, 64), "f16", through="f16")
+    close(got[keep_rows][:, keep], want[:, keep], bound[:, keep])
+    # behind the last column stands what is not the product's: rows of a wider tensor
+    x[3, 5] = x[4, 6] = 0
+    x[:, :5] = np.nan
+    back = give(wgf, dev, np.concatenate([x[:, 5:], x[:, :5]], 1), "f16").slice([(0, rows), (0, k)]).mat_mul_q4(t)
+    assert np.isfinite(np.asarray(take(back, "f16"))[:, keep]).all()
+
+
+def test_q4_product_on_tensor_cores_replayed(wgf, dev):
+    g = seeded(29, 2)
+    rows, n, k = 300, 1100, 1100
+    w, x = draw(g, (n, k), "bf16", 0.02), draw(g, (rows, k), "bf16")
+    t, a = give(wgf, dev, w, "bf16").quantize_q4(64), give(wgf, dev, x, "bf16")
+    want = take(a.mat_mul_q4(t), "bf16")
+    with dev.record() as s:
+        out = a.mat_mul_q4(t).materialize()
+    for _ in range(3):
+        s.launch()
+    np.testing.assert_array_equal(take(out, "bf16"), want)
 
 
 @pytest.mark.parametrize("kind", ["f32", "f16"])

@@ -21,14 +21,16 @@
 // measured rate of memory); 16.5 with a CTA for each row tile, whose first loads, staging of x and sums were not
 // overlapped with anything, and 22 where a scale was converted, and so waited for, in the turn that called for it.
 // Seven rows of bf16 through 4096 x 11008: 14.4 us.
-// More rows: in blocks, along the grid's second axis.  Many rows: the weights are written out in the type of x once and
-// the matrix product kernels take them (rows_in_blocks has both sides' times).
+// More rows: in blocks, along the grid's second axis, on the tensor cores (q4_tc.cu), or with the weights written out in the type of
+// x for the matrix product kernels (choose_way has the times).
 #include <algorithm>
+#include <cmath>
 
 #include <cooperative_groups.h>
 
 #include "decode.hpp"
 #include "decode_common.cuh"
+#include "q4_tc.hpp"
 
 namespace wgf {
 
@@ -130,29 +132,57 @@ __global__ void q4_pack_scales_kernel(const U* __restrict__ in, U* __restrict__ 
     }
 }
 
-// The values that the codes stand for, row by row.  A thread has one word: four columns of two rows.
+// The values that the codes stand for, row by row, zeros between the last column and the end of a padded row.  A warp has tiles
+// of kSpan chunks in a row, a lane eight columns of rows g and g + 8 at a time.  11008 x 4096 as f16: 28 us; with a thread for each
+// word, whose place took four divisions of 64 bits, 52.
+constexpr int kSpan = 4;
 template <typename T>
-__global__ void q4_dequantize_kernel(const uint32_t* __restrict__ codes, const void* __restrict__ scales, DType sdt, T* __restrict__ out, long long n,
-                                     long long k, long long stride, int group, long long chunks, long long groups, long long words) {
-    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < words; i += (long long)gridDim.x * blockDim.x) {
-        // neighbours write neighbouring columns
-        const int c = (int)(i >> 1) & 3, st = (int)(i >> 3 & 1) * 2 + (int)(i & 1), g = (int)(i >> 4) & 7;
-        const long long tile = i >> 7, rt = tile / chunks, col = (tile % chunks) * 64 + (i & 15) * 4;
-        const unsigned w = codes[tile * 128 + (g * 4 + c) * 4 + st];
-        if (col >= stride) continue;                        // zeros between the last column and the end of a padded row
-        const long long q = min(col / group, groups - 1);
+__global__ void q4_dequantize_kernel(const uint4* __restrict__ codes, const void* __restrict__ scales, DType sdt, T* __restrict__ out, long long n,
+                                     long long k, long long stride, int group_log2, long long chunks, long long groups, long long spans, long long jobs) {
+    typedef Pack<T, 16 / (int)sizeof(T)> V;
+    constexpr int PER = 16 / (int)sizeof(T);
+    const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    const bool wide = stride % PER == 0;
+    for (long long job = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); job < jobs; job += (long long)gridDim.x * (blockDim.x >> 5)) {
+        const long long rt = job / spans, first = (job - rt * spans) * kSpan, row = rt * 16 + g;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const long long row = rt * 16 + g + half * 8;
-            if (row >= n) continue;
-            const float s = scale_at(scales, sdt, (rt * groups + q) * 16 + scale_slot(g + half * 8));
-            Pack<T, 4> v;
+        for (int i = 0; i < kSpan; ++i) {
+            const long long chunk = first + i;
+            if (chunk >= chunks) break;
+            const uint4 w = codes[(rt * chunks + chunk) * 32 + lane];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v.v[e] = from_f<T>(col + e < k ? (float)((int)((w >> (4 * nibble(half, e))) & 15u) - 8) * s : 0.f);
-            T* to = out + row * stride + col;
-            if (stride % 4 == 0) *reinterpret_cast<Pack<T, 4>*>(to) = v;
-            else
-                for (int e = 0; e < 4 && col + e < stride; ++e) to[e] = v.v[e];
+            for (int half = 0; half < 2; ++half) {
+                const long long col = chunk * 64 + half * 32 + c * 8;
+                if (col >= stride) continue;
+                const unsigned word[2] = {half ? w.z : w.x, half ? w.w : w.y};
+                const long long q = min(col >> group_log2, groups - 1);
+#pragma unroll
+                for (int low = 0; low < 2; ++low) {
+                    if (row + low * 8 >= n) continue;
+                    const float s = scale_at(scales, sdt, (rt * groups + q) * 16 + g * 2 + low);
+                    T v[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = from_f<T>((float)((int)((word[e >> 2] >> (4 * nibble(low, e & 3))) & 15u) - 8) * s);
+                    if (col + 8 > k)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (col + e >= k) v[e] = from_f<T>(0.f);
+                    T* to = out + (row + low * 8) * stride + col;
+                    if (wide && col + 8 <= stride) {
+#pragma unroll
+                        for (int e = 0; e < 8; e += PER) {
+                            V p;
+#pragma unroll
+                            for (int f = 0; f < PER; ++f) p.v[f] = v[e + f];
+                            *reinterpret_cast<V*>(to + e) = p;
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (col + e < stride) to[e] = v[e];
+                    }
+                }
+            }
         }
     }
 }
@@ -632,6 +662,8 @@ Q4Ref q4_from_host(const DeviceRef& devref, int64_t n, int64_t k, int64_t group,
     return w;
 }
 
+static int group_log2(const Q4Weight& w) { return w.group == 32 ? 5 : w.group == 64 ? 6 : 7; }
+
 // [n, k] in rows of `stride` elements, zeros behind the last column
 static TensorData dequantize_rows(Device& dev, const Q4Weight& w, DType dtype, int64_t stride) {
     dev.make_current();
@@ -641,13 +673,13 @@ static TensorData dequantize_rows(Device& dev, const Q4Weight& w, DType dtype, i
     out.dtype = dtype;
     out.layout = Layout::contiguous({w.n, stride});
     out.buf = dev.alloc((size_t)(w.n * stride) * dtype_size(dtype), false);
-    const long long words = w.row_tiles * w.chunks * 128;
+    const long long spans = (w.chunks + kSpan - 1) / kSpan, jobs = w.row_tiles * spans;
     auto go = [&](auto zero) {
         typedef decltype(zero) T;
         dev.begin_launch("q4_dequantize");
         if (!dev.dry)
-            q4_dequantize_kernel<T><<<grid_for(dev, words), 256, 0, dev.stream>>>((const uint32_t*)w.codes->ptr, w.scales->ptr, w.scale_dtype,
-                (T*)out.buf->ptr, w.n, w.k, stride, (int)w.group, w.chunks, w.groups, words);
+            q4_dequantize_kernel<T><<<grid_for(dev, jobs * 32), 256, 0, dev.stream>>>((const uint4*)w.codes->ptr, w.scales->ptr, w.scale_dtype,
+                (T*)out.buf->ptr, w.n, w.k, stride, group_log2(w), w.chunks, w.groups, spans, jobs);
         dev.end_launch();
     };
     if (dtype == DType::F32) go(0.f);
@@ -687,15 +719,21 @@ static RowsPlan plan_rows(Device& dev, const Q4Weight& w, int64_t rows, int part
     return best;
 }
 
-// Whether rows go through the kernel above in blocks, or through weights that are written out and the matrix product.
-// Rows of 16 bits: the tensor-core product takes 64 rows at least (fewer run strided: 640 us for 16 rows through
-// 11008 x 4096, 19 in blocks); from there on both sides are estimated.  In us, blocks against weights written out:
-// 11008 x 4096: 80 rows 76 / 80, 100 rows 82 / 80; 4096 x 4096: 80 rows 27 / 43, 128 rows 56 / 43; 600 x 900: 200 rows 13 / 19.
-// Rows of f32: the FFMA product is slow for rows like these: 4096 x 4096: 500 rows 501 / 615; 11008 x 4096: 500 rows 1308 / 1562.
-static bool rows_in_blocks(const RowsPlan& plan, const Q4Weight& w, int64_t rows, int parts) {
-    if (!plan.shares) return false;
-    if (parts > 1) return rows <= 512;
-    return rows < 64 || 3.0 + 0.021 * plan.cost < 12.0 + 0.005 * (double)w.k + 1.1e-6 * (double)w.n * (double)w.k;
+// Which way rows take: in blocks through the kernel above, through the tensor cores (q4_tc.cu), or through weights that are
+// written out and the matrix product.  Rows of 16 bits: what each would take is estimated, in us.  Measured, blocks / tensor
+// cores / written out: 11008 x 4096, 40 rows 38 / 36 / 660 (the matrix product of fewer than 64 rows is strided), 64 rows 80 / 36 / 63,
+// 128 rows 118 / 39 / 63, 500 rows 380 / 73 / 80, 1000 rows 722 / 105 / 107, 2048 rows 1450 / 163 / 145; 4096 x 4096, 40 rows 24 / 36 / -,
+// 64 rows 39 / 36 / 42, 800 rows 283 / 46 / 45; 1024 x 1024, 64 rows 11 / 15 / 23, 500 rows 28 / 16 / 26.
+// Rows of f32 have no tensor-core form, and the FFMA product is slow for rows like these: 4096 x 4096: 500 rows 501 in blocks, 615
+// written out; 11008 x 4096: 500 rows 1308 / 1562.
+enum class Q4Way { BLOCKS, TENSOR, WRITTEN };
+static Q4Way choose_way(Device& dev, const RowsPlan& plan, const Q4TcPlan& tc, const Q4Weight& w, int64_t rows, int parts) {
+    if (parts > 1) return plan.shares && rows <= 512 ? Q4Way::BLOCKS : Q4Way::WRITTEN;
+    const double blocks = plan.shares ? 3.0 + 0.021 * plan.cost : 1e30;
+    // the matrix product: tiles of 256 x 256 for a pair of SMs, of which half a wave can be cut smaller
+    const double tiles = (double)((rows + 255) / 256) * (double)((w.n + 255) / 256), waves = std::max(1.0, std::ceil(2.0 * tiles / (dev.sm_count / 2)) / 2);
+    const double written = rows < 64 ? 1e30 : 3.0 + 0.55e-6 * (double)w.n * (double)w.k + 8.0 + 0.43 * waves * (double)w.chunks;
+    return blocks <= std::min(tc.us, written) ? Q4Way::BLOCKS : tc.us <= written ? Q4Way::TENSOR : Q4Way::WRITTEN;
 }
 
 TensorData run_matmul_q4(Device& dev, const TensorData& x_in, const Q4Weight& w) {
@@ -718,11 +756,14 @@ TensorData run_matmul_q4(Device& dev, const TensorData& x_in, const Q4Weight& w)
     dev.wait_for(*x.buf);
     const int parts = x.dtype == DType::F32 ? 3 : 1;
     const RowsPlan plan = plan_rows(dev, w, rows, parts);
-    if (!rows_in_blocks(plan, w, rows, parts)) {
-        // in rows of whole 16 bytes, which the tensor-core kernels want of both operands
+    const Q4TcPlan tc = q4_tc_plan(dev, w, rows);
+    const Q4Way way = choose_way(dev, plan, tc, w, rows, parts);
+    dev.note_recorded_buffer(w.codes);
+    dev.note_recorded_buffer(w.scales);
+    if (way != Q4Way::BLOCKS) {
+        // rows that begin at 16-byte borders, which the tensor-core kernels want
         const int64_t kp = parts == 1 ? (w.k + 7) / 8 * 8 : w.k;
-        TensorData full = dequantize_rows(dev, w, x.dtype, kp);
-        if (kp != w.k) {
+        if (parts == 1 && (kp != w.k || x.layout.strides[1] != 1 || x.layout.strides[0] % 8 || x.layout.strides[0] < w.k || (uintptr_t)x.base_ptr() % 16)) {
             TensorData wide;
             wide.dtype = x.dtype;
             wide.layout = Layout::contiguous({rows, kp});
@@ -732,14 +773,18 @@ TensorData run_matmul_q4(Device& dev, const TensorData& x_in, const Q4Weight& w)
             run_copy(dev, window, x);
             x = wide;
         }
+        if (way == Q4Way::TENSOR) {
+            out.buf = dev.alloc((size_t)(rows * w.n) * dtype_size(x.dtype), false);
+            if (q4_tc_run(dev, w, tc, x, rows, out.base_ptr())) return out;
+        }
+        x.layout.shape = {rows, kp};
+        TensorData full = dequantize_rows(dev, w, x.dtype, kp);
         full.layout.shape = {kp, w.n};
         full.layout.strides = {1, kp};
         TensorData y = run_matmul(dev, x, full);
         y.layout = out.layout;
         return y;
     }
-    dev.note_recorded_buffer(w.codes);
-    dev.note_recorded_buffer(w.scales);
     if (x.layout.strides[1] != 1 && w.k > 1) x = run_compact(dev, x);
     out.buf = dev.alloc((size_t)(rows * w.n) * dtype_size(x.dtype), false);
     Q4Params p{};
@@ -755,7 +800,7 @@ TensorData run_matmul_q4(Device& dev, const TensorData& x_in, const Q4Weight& w)
     p.columns = plan.block_rows * parts;
     p.chunks = (int)w.chunks;
     p.groups = (int)w.groups;
-    p.group_log2 = w.group == 32 ? 5 : w.group == 64 ? 6 : 7;
+    p.group_log2 = group_log2(w);
     p.row_tiles = (int)w.row_tiles;
     p.scale_dtype = w.scale_dtype;
     p.tiles = plan.tiles;

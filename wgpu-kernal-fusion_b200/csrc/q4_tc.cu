@@ -1,0 +1,428 @@
+// Products with 4-bit weights for many rows of f16 or bf16, on the tensor cores.
+//
+//   y[m, n] = sum_k x[m, k] w[n, k],   w[n, k] = scale[n, k / group] * (code[n, k] - 8), rounded once to the type of x
+//
+// The weights are the A operand: a tile is 128 of their rows by up to 256 rows of x, whose number is chosen so that the tiles
+// fill the SMs (q4_tc_plan).  Warp roles of a CTA, one CTA a SM:
+//   warp 0       brings x by TMA: 64 columns of all rows of the tile, 128-byte swizzle
+//   warp 1       issues tcgen05.mma (M = 128, N = the tile's rows of x, K = 16) into two accumulators in tensor memory in turn
+//   warps 2-5    write finished accumulators out: a lane is a row of the weights, so a warp writes 32 neighbours of a row of y
+//   warps 6-21   turn codes into the operand: 16 rows by 64 columns are 512 bytes, 16 to a lane, whose words are eight columns in a
+//                row of rows g and g + 8 (q4.cu): four 16-byte stores, where the swizzle wants them.  Odd g take the two
+//                halves in the other order, so that the lanes of a store fall on different banks.
+//   warp 22      brings the codes and scales of two steps at a time by bulk copies
+// Every wait is bounded and reports through the device's error word.
+// 500 rows of f16 through 11008 x 4096: 67 us in two waves of tiles of 176 rows, where weights written out and the matrix product take
+// 76 together, and the products alone 27 at the measured rate of the tensor cores; 100 rows 35 us against 58.  A step of 64
+// columns takes 0.4 us with few rows of x and 0.5 with 256, while its products take 0.05 to 0.39: turning the codes into the operand, the
+// copies and the handing over of a step cost about 0.2 us each and overlap only in part (without the first 0.33, without all of them
+// 0.2), and with 256 rows L2 delivers x at about 9 TB/s.  Tried and not kept: 256 rows of weights a tile (half the traffic of x, one wave
+// of 500 rows: 74 us), two steps to a stage (72), two CTAs a SM with half the decoders (69), one lane that waits for its warp (115).
+#include <algorithm>
+#include <type_traits>
+
+#include "decode.hpp"
+#include "decode_common.cuh"
+#include "q4_tc.hpp"
+#include "tc_common.cuh"
+
+namespace wgf {
+
+using namespace tc;
+using decode::shared_16;
+using decode::shared_float2;
+using decode::shared_word;
+
+namespace {
+
+constexpr int kBK = 64;                  // columns of a step
+constexpr int kDecoders = 16;            // warps; eight have the even steps of a tile and eight the odd ones
+constexpr int kThreadsTc = (7 + kDecoders) * 32;
+constexpr int kPairs = 4;                // pairs of steps whose codes are on their way
+constexpr int kMaxStages = 8;
+constexpr int kWBytes = 128 * kBK * 2;   // of a stage: the weights' part
+constexpr int kRoom = 225 * 1024;        // shared memory of all stages and pairs
+
+struct Q4TcParams {
+    const uint4* codes;
+    const void* scales;
+    void* y;
+    long long n, rows, k;
+    int chunks, groups, group_log2, row_tiles;
+    DType scale_dtype;
+    int tile_rows;                       // of x
+    int tiles_m, tiles_n, stages;
+    int scale_bytes, tile_bytes;         // of a scale; of a tile of 16 rows in a pair of steps
+    unsigned* error;
+};
+
+// fp32 accumulator, both operands K-major f16 or bf16, M = 128, N = rows
+__device__ __forceinline__ unsigned instruction(bool bf16, int rows) {
+    return (1u << 4) | (bf16 ? 1u << 7 | 1u << 10 : 0u) | (unsigned)(rows >> 3) << 17 | (128u >> 4) << 24;
+}
+
+// What a lane needs of a tile of 16 rows by 64 columns: its words, and as they are stored the scales of rows g and g + 8 for
+// each group.  SAME: scales of the type of x, two in a word.
+template <bool G32> struct Q4Unit {
+    uint4 w;
+    uint2 s[G32 ? 2 : 1];
+};
+
+// Two codes 16 bits apart as two values of the type, times the scale: code - 8 is exact, the product is rounded once
+template <typename T> struct TwoOf;
+template <> struct TwoOf<__half> { typedef __half2 type; };
+template <> struct TwoOf<__nv_bfloat16> { typedef __nv_bfloat162 type; };
+// The nibbles of rows g stand at bit 0 of `nib`, those of rows g + 8 at bit 4.
+template <typename T, bool LOW> __device__ __forceinline__ typename TwoOf<T>::type less_eight(unsigned nib) {
+    if constexpr (std::is_same<T, __half>::value) {
+        const unsigned v = (nib & (LOW ? 0x00f000f0u : 0x000f000fu)) | 0x64006400u;          // 1024 + code, or + 16 code
+        const __half2 f = *reinterpret_cast<const __half2*>(&v);
+        if constexpr (LOW) return __hfma2(f, __half2half2(__ushort_as_half(0x2c00)), __half2half2(__ushort_as_half(0xd480)));
+        else return __hsub2(f, __half2half2(__ushort_as_half(0x6408)));
+    } else {
+        const unsigned v = ((LOW ? nib >> 4 : nib) & 0x000f000fu) | 0x43004300u;             // 128 + code
+        return __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), __bfloat162bfloat162(__ushort_as_bfloat16(0x4308)));
+    }
+}
+template <typename T, bool SAME, bool LOW> __device__ __forceinline__ unsigned two_values(unsigned nib, typename TwoOf<T>::type s2, float s) {
+    const auto d = less_eight<T, LOW>(nib);
+    if constexpr (SAME) {
+        const auto v = __hmul2(d, s2);
+        return *reinterpret_cast<const unsigned*>(&v);
+    } else {
+        return pack2<T>(__low2float(d) * s, __high2float(d) * s);
+    }
+}
+__device__ __forceinline__ __half2 two_low(__half2 v) { return __low2half2(v); }
+__device__ __forceinline__ __half2 two_high(__half2 v) { return __high2half2(v); }
+__device__ __forceinline__ __nv_bfloat162 two_low(__nv_bfloat162 v) { return __low2bfloat162(v); }
+__device__ __forceinline__ __nv_bfloat162 two_high(__nv_bfloat162 v) { return __high2bfloat162(v); }
+// The values behind the row's end are zero whatever the scale is
+__device__ __forceinline__ uint4 first_of(uint4 v, int valid) {
+    unsigned* r = reinterpret_cast<unsigned*>(&v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (valid <= 2 * i) r[i] = 0;
+        else if (valid == 2 * i + 1) r[i] &= 0xffffu;
+    return v;
+}
+// From global to shared memory, both from 16-byte borders on and in multiples of 16 bytes
+__device__ __forceinline__ void bulk_load(unsigned dst, const void* src, unsigned bytes, unsigned bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+                 : "memory");
+}
+__device__ __forceinline__ void store16(unsigned at, uint4 v) {
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+// A unit as the operand.  `at`: the lane's place for the first of the two halves of a row that it writes; the other is 64
+// bytes away.  `valid`, where the row ends in the unit (ENDS): columns from the lane's first on in the first half.
+template <typename T, bool SAME, bool G32, bool ENDS>
+__device__ __forceinline__ void decode_unit(const Q4Unit<G32>& u, DType scale_dtype, bool odd, unsigned at, int valid) {
+    typedef typename TwoOf<T>::type T2;
+    const unsigned words[4] = {odd ? u.w.z : u.w.x, odd ? u.w.w : u.w.y, odd ? u.w.x : u.w.z, odd ? u.w.y : u.w.w};
+#pragma unroll
+    for (int turn = 0; turn < 2; ++turn) {
+        const unsigned a = words[2 * turn], b = words[2 * turn + 1];
+        uint2 raw = u.s[0];
+        if (G32) raw = (turn == 0) == odd ? u.s[G32 ? 1 : 0] : raw;
+        T2 up{}, low{};
+        float fu = 0.f, fl = 0.f;
+        if constexpr (SAME) {
+            const T2 both = *reinterpret_cast<const T2*>(&raw.x);
+            up = two_low(both);
+            low = two_high(both);
+        } else if (scale_dtype == DType::F32) {
+            fu = __uint_as_float(raw.x);
+            fl = __uint_as_float(raw.y);
+        } else if (scale_dtype == DType::F16) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&raw.x));
+            fu = f.x;
+            fl = f.y;
+        } else {
+            fu = __uint_as_float(raw.x << 16);
+            fl = __uint_as_float(raw.x & 0xffff0000u);
+        }
+        const unsigned a8 = a >> 8, b8 = b >> 8;
+        uint4 top = make_uint4(two_values<T, SAME, false>(a, up, fu), two_values<T, SAME, false>(a8, up, fu), two_values<T, SAME, false>(b, up, fu),
+                               two_values<T, SAME, false>(b8, up, fu));
+        uint4 bottom = make_uint4(two_values<T, SAME, true>(a, low, fl), two_values<T, SAME, true>(a8, low, fl), two_values<T, SAME, true>(b, low, fl),
+                                  two_values<T, SAME, true>(b8, low, fl));
+        if (ENDS) {
+            const int left = valid - 32 * (turn ^ (int)odd);
+            top = first_of(top, left);
+            bottom = first_of(bottom, left);
+        }
+        store16(turn ? at ^ 64u : at, top);
+        store16((turn ? at ^ 64u : at) + 1024, bottom);
+    }
+}
+
+template <typename T, bool SAME, bool G32>
+__global__ void __launch_bounds__(kThreadsTc, 1) q4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ Q4TcParams p) {
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ alignas(8) unsigned long long bars[3 * kMaxStages + 4 + 2 * kPairs];
+    __shared__ unsigned tmem_slot;
+    const unsigned stages_at = (smem_u32(smem_raw) + 1023) & ~1023u;          // the swizzle wants 1024-byte alignment
+    const unsigned stage_bytes = kWBytes + (unsigned)p.tile_rows * kBK * 2;
+    const unsigned pairs_at = stages_at + p.stages * stage_bytes, pair_bytes = 8u * p.tile_bytes;
+    const unsigned bar0 = smem_u32(bars);
+    auto x_full = [&](int s) { return bar0 + 8u * s; };
+    auto w_full = [&](int s) { return bar0 + 8u * (kMaxStages + s); };
+    auto empty = [&](int s) { return bar0 + 8u * (2 * kMaxStages + s); };
+    auto acc_full = [&](int a) { return bar0 + 8u * (3 * kMaxStages + a); };
+    auto acc_empty = [&](int a) { return bar0 + 8u * (3 * kMaxStages + 2 + a); };
+    auto pair_full = [&](int b) { return bar0 + 8u * (3 * kMaxStages + 4 + b); };
+    auto pair_empty = [&](int b) { return bar0 + 8u * (3 * kMaxStages + 4 + kPairs + b); };
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kMaxStages; ++s) {
+            mbar_init(x_full(s), 1);
+            mbar_init(w_full(s), 8);
+            mbar_init(empty(s), 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(acc_full(a), 1);
+            mbar_init(acc_empty(a), 4);
+        }
+        for (int b = 0; b < kPairs; ++b) {
+            mbar_init(pair_full(b), 1);
+            mbar_init(pair_empty(b), kDecoders);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) tmem_alloc(smem_u32(&tmem_slot), 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const unsigned tmem = tmem_slot;
+    const int tiles = p.tiles_m * p.tiles_n;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int stage = 0;
+            unsigned phase = 1;                       // a fresh barrier counts as released
+            bool ok = true;
+            for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+                const int m0 = tile % p.tiles_m * p.tile_rows;
+                for (int kb = 0; kb < p.chunks; ++kb) {
+                    if (!mbar_wait(empty(stage), phase)) {
+                        atomicExch(p.error, 11u);
+                        ok = false;
+                        break;
+                    }
+                    mbar_expect_tx(x_full(stage), (unsigned)p.tile_rows * kBK * 2);
+                    tma_load_3d(stages_at + stage * stage_bytes + kWBytes, &map_x, x_full(stage), kb * kBK, m0, 0);
+                    if (++stage == p.stages) stage = 0, phase ^= 1;
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            const unsigned idesc = instruction(std::is_same<T, __nv_bfloat16>::value, p.tile_rows);
+            const unsigned long long first = smem_desc(stages_at, 16, 1024);      // its addresses are in units of 16 bytes
+            int stage = 0, acc = 0;
+            unsigned phase = 0, acc_phase = 1;
+            bool ok = true;
+            for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+                if (!mbar_wait(acc_empty(acc), acc_phase)) {
+                    atomicExch(p.error, 12u);
+                    break;
+                }
+                tc_fence_after();
+                for (int kb = 0; kb < p.chunks; ++kb) {
+                    if (!mbar_wait(x_full(stage), phase) || !mbar_wait(w_full(stage), phase)) {
+                        atomicExch(p.error, 13u);
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const unsigned long long w = first + (unsigned)stage * (stage_bytes >> 4), x = w + (kWBytes >> 4);
+#pragma unroll
+                    for (int i = 0; i < kBK / 16; ++i) umma_f16(tmem + (unsigned)acc * 256, w + 2 * i, x + 2 * i, idesc, (kb | i) != 0);
+                    umma_commit(empty(stage));
+                    if (++stage == p.stages) stage = 0, phase ^= 1;
+                }
+                if (ok) umma_commit(acc_full(acc));
+                if (++acc == 2) acc = 0, acc_phase ^= 1;
+            }
+        }
+    } else if (warp < 6) {
+        const int quarter = warp & 3;                 // of the accumulator's lanes
+        int acc = 0;
+        unsigned acc_phase = 0;
+        for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+            if (!mbar_wait(acc_full(acc), acc_phase)) {
+                if (lane == 0) atomicExch(p.error, 14u);
+                break;
+            }
+            tc_fence_after();
+            const long long m0 = (long long)(tile % p.tiles_m) * p.tile_rows;
+            const int live = (int)min((long long)p.tile_rows, p.rows - m0);
+            const long long n = (long long)(tile / p.tiles_m) * 128 + quarter * 32 + lane;
+            T* to = (T*)p.y + m0 * p.n + n;
+            for (int c = 0; c < live; c += 32) {
+                unsigned v[32];
+                tmem_ld_32x32(tmem + ((unsigned)(quarter * 32) << 16) + (unsigned)(acc * 256 + c), v);
+                tmem_ld_wait();
+                if (n < p.n) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if (c + j < live) to[(c + j) * p.n] = decode::from_f<T>(__uint_as_float(v[j]));
+                }
+                __syncwarp();
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(acc_empty(acc));
+            if (++acc == 2) acc = 0, acc_phase ^= 1;
+        }
+    } else if (warp < 6 + kDecoders) {
+        const int d = (warp - 6) & 7, odd = (warp - 6) >> 3;
+        // where this lane's words, scales and places in the operand are in a pair and a stage
+        const unsigned words = pairs_at + d * p.tile_bytes + odd * 512 + lane * 16;
+        const unsigned scales = pairs_at + d * p.tile_bytes + 1024 + (((odd * 64) >> p.group_log2) * 16 + (lane >> 2) * 2) * p.scale_bytes;
+        const int g = lane >> 2, c = lane & 3;
+        const unsigned operand = stages_at + (d * 16 + g) * 128 + (((g & 1) * 4 + c) ^ g) * 16;
+        int stage = 0, buffer = 0;
+        unsigned phase = 1, pair_phase = 0;
+        bool ok = true;
+        for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x)
+            for (int kb = 0; kb < p.chunks; kb += 2) {
+                int s = stage + odd;
+                unsigned s_phase = phase;
+                if (s >= p.stages) s -= p.stages, s_phase ^= 1;
+                const bool live = kb + odd < p.chunks;
+                if (!mbar_wait(pair_full(buffer), pair_phase) || (live && !mbar_wait(empty(s), s_phase))) {
+                    if (lane == 0) atomicExch(p.error, 15u);
+                    ok = false;
+                    break;
+                }
+                if (live) {
+                    Q4Unit<G32> u;
+                    u.w = shared_16(words + buffer * pair_bytes);
+#pragma unroll
+                    for (int i = 0; i < (G32 ? 2 : 1); ++i) {
+                        const unsigned at = scales + buffer * pair_bytes + i * 16 * p.scale_bytes;
+                        if (!SAME && p.scale_bytes == 4) {
+                            const float2 f = shared_float2(at);
+                            u.s[i] = make_uint2(__float_as_uint(f.x), __float_as_uint(f.y));
+                        } else {
+                            u.s[i].x = shared_word(at);
+                        }
+                    }
+                    const unsigned at = operand + s * stage_bytes;
+                    const int valid = (int)p.k - (kb + odd) * kBK - c * 8;
+                    if (valid + c * 8 >= kBK) decode_unit<T, SAME, G32, false>(u, p.scale_dtype, g & 1, at, valid);
+                    else decode_unit<T, SAME, G32, true>(u, p.scale_dtype, g & 1, at, valid);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                }
+                __syncwarp();
+                if (lane == 0) {
+                    if (live) mbar_arrive(w_full(s));
+                    mbar_arrive(pair_empty(buffer));
+                }
+                stage += min(2, p.chunks - kb);
+                if (stage >= p.stages) stage -= p.stages, phase ^= 1;
+                if (++buffer == kPairs) buffer = 0, pair_phase ^= 1;
+            }
+    } else {
+        int buffer = 0;
+        unsigned phase = 1;
+        bool ok = true;
+        for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+            // tiles behind the last are the last again: nobody reads what becomes of their rows
+            const long long rt = min(tile / p.tiles_m * 8 + (lane & 7), p.row_tiles - 1);
+            const uint4* words = p.codes + rt * p.chunks * 32;
+            const unsigned char* scales = (const unsigned char*)p.scales + rt * p.groups * 16 * p.scale_bytes;
+            for (int kb = 0; kb < p.chunks; kb += 2) {
+                if (!mbar_wait(pair_empty(buffer), phase)) {
+                    if (lane == 0) atomicExch(p.error, 16u);
+                    ok = false;
+                    break;
+                }
+                const int q = kb * 64 >> p.group_log2;
+                const unsigned wb = min(2, p.chunks - kb) * 512u, sb = min(128 >> p.group_log2, p.groups - q) * 16u * p.scale_bytes;
+                if (lane == 0) mbar_expect_tx(pair_full(buffer), 8 * (wb + sb));
+                __syncwarp();
+                if (lane < 8) {
+                    const unsigned to = pairs_at + buffer * pair_bytes + lane * p.tile_bytes;
+                    bulk_load(to, words + kb * 32, wb, pair_full(buffer));
+                    bulk_load(to + 1024, scales + q * 16 * p.scale_bytes, sb, pair_full(buffer));
+                }
+                if (++buffer == kPairs) buffer = 0, phase ^= 1;
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+}  // namespace
+
+// Tiles of few rows of x cost nearly what tiles of many do, as the time goes into the weights' side: so as few waves as 256 rows
+// allow, and of those the smallest tiles.  In us: a step of 64 columns takes 0.44 with 64 rows of x, 0.47 with 128, 0.55 with 256.
+Q4TcPlan q4_tc_plan(Device& dev, const Q4Weight& w, int64_t rows) {
+    Q4TcPlan best;
+    const int64_t tiles_n = (w.row_tiles + 7) / 8, least = (rows + 255) / 256;
+    for (int64_t t = least; t < least + 16; ++t) {
+        const int64_t tile_rows = ((rows + t - 1) / t + 15) / 16 * 16;
+        const int64_t waves = (tiles_n * t + dev.sm_count - 1) / dev.sm_count;
+        const double us = 5.0 + (double)waves * (double)w.chunks * (0.40 + 0.0006 * (double)tile_rows);
+        if (us < best.us) best = {(int)tile_rows, us};
+    }
+    return best;
+}
+
+bool q4_tc_run(Device& dev, const Q4Weight& w, const Q4TcPlan& plan, const TensorData& x, int64_t rows, void* y) {
+    const bool bf16 = x.dtype == DType::BF16;
+    const int64_t stride = x.layout.strides[0];
+    CUtensorMap map;
+    if (!dev.dry && !encode_3d(&map, bf16, x.base_ptr(), w.k, rows, 1, stride, rows * stride, kBK, (unsigned)plan.tile_rows)) return false;
+    Q4TcParams p{};
+    p.codes = (const uint4*)w.codes->ptr;
+    p.scales = w.scales->ptr;
+    p.y = y;
+    p.n = w.n;
+    p.rows = rows;
+    p.k = w.k;
+    p.chunks = (int)w.chunks;
+    p.groups = (int)w.groups;
+    p.group_log2 = w.group == 32 ? 5 : w.group == 64 ? 6 : 7;
+    p.row_tiles = (int)w.row_tiles;
+    p.scale_dtype = w.scale_dtype;
+    p.tile_rows = plan.tile_rows;
+    p.tiles_m = (int)((rows + plan.tile_rows - 1) / plan.tile_rows);
+    p.tiles_n = (int)((w.row_tiles + 7) / 8);
+    p.scale_bytes = (int)dtype_size(w.scale_dtype);
+    p.tile_bytes = 1024 + (int)(128 / w.group) * 16 * p.scale_bytes;
+    const int stage_bytes = kWBytes + plan.tile_rows * kBK * 2, pairs_bytes = kPairs * 8 * p.tile_bytes;
+    p.stages = std::min(kMaxStages, (kRoom - pairs_bytes) / stage_bytes);
+    p.error = dev.error_word();
+    const unsigned grid = (unsigned)std::min<int64_t>((int64_t)p.tiles_m * p.tiles_n, dev.sm_count);
+    const int smem = p.stages * stage_bytes + pairs_bytes + 1024;
+    dev.begin_launch("q4_tc");
+    if (!dev.dry) {
+        auto go = [&](auto kernel) {
+            WGF_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRoom + 1024));
+            kernel<<<grid, kThreadsTc, smem, dev.stream>>>(map, p);
+        };
+        const bool same = w.scale_dtype == x.dtype, g32 = w.group == 32;
+        if (bf16) {
+            if (same) g32 ? go(q4_tc_kernel<__nv_bfloat16, true, true>) : go(q4_tc_kernel<__nv_bfloat16, true, false>);
+            else g32 ? go(q4_tc_kernel<__nv_bfloat16, false, true>) : go(q4_tc_kernel<__nv_bfloat16, false, false>);
+        } else {
+            if (same) g32 ? go(q4_tc_kernel<__half, true, true>) : go(q4_tc_kernel<__half, true, false>);
+            else g32 ? go(q4_tc_kernel<__half, false, true>) : go(q4_tc_kernel<__half, false, false>);
+        }
+    }
+    dev.end_launch();
+    return true;
+}
+
+}  // namespace wgf
