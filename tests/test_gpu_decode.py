@@ -307,6 +307,50 @@ def test_cache_beyond_four_gigabytes(wgf, dev):
     assert not out[1].any()
 
 
+def test_cache_of_many_sequences(wgf, dev):
+    """More sequences than a launch takes counts by value, and taken back, appended to and attended to by counts."""
+    g = seeded(22, 95)
+    b, t = 301, 70
+    lens = [int(n) for n in g.integers(0, t + 1, b)]
+    k, v = draw(g, (b, 1, t, 8), "f16", 2.0), draw(g, (b, 1, t, 8), "f16", 2.0)
+    c = dev.kv_cache(b, 1, 8, t + 9, wgf.F16)
+    tk, tv = give(wgf, dev, k, "f16"), give(wgf, dev, v, "f16")
+    c.append(tk, tv, counts=lens)
+    back = [max(n - int(d), 0) for n, d in zip(lens, g.integers(0, 3, b))]
+    c.truncate(back)
+    more = [int(n) for n in g.integers(0, 5, b)]
+    nk, nv = draw(g, (b, 1, 4, 8), "f16", 2.0), draw(g, (b, 1, 4, 8), "f16", 2.0)
+    c.append(give(wgf, dev, nk, "f16"), give(wgf, dev, nv, "f16"), counts=more)
+    assert c.lengths == [n + m for n, m in zip(back, more)]
+    both = [[np.concatenate([x[i, 0, :n], y[i, 0, :m]]) for i, (n, m) in enumerate(zip(back, more))] for x, y in ((k, nk), (v, nv))]
+    for got, want in zip(c.read(), both):
+        got = take(got, "f16")
+        for i, x in enumerate(want):
+            np.testing.assert_array_equal(got[i, 0, : len(x)], ref.round_to(ref.stands_for(x), "f16"))
+            assert not got[i, 0, len(x):].any()
+    q = draw(g, (b, 2, 4, 8), "f16")
+    out = take(c.attention(give(wgf, dev, q, "f16"), counts=more), "f16")
+    for i in range(b):
+        want, bound = ref.attention(q[i], *(ref.stands_for(x[i])[None] for x in both), 8 ** -0.5, more[i])
+        close(out[i], want, bound + ref.rounding(want, "f16"))
+
+
+def test_cache_attention_of_very_many_jobs(wgf, dev):
+    """More sequences times heads than there are tickets to join parts with."""
+    g = seeded(22, 94)
+    b, heads = 8300, 8
+    lens = [int(n) for n in g.integers(0, 4, b)]
+    lens[17], lens[b - 1] = 64, 61
+    k, v, q = draw(g, (b, heads, 64, 8), "f16"), draw(g, (b, heads, 64, 8), "f16"), draw(g, (b, heads, 1, 8), "f16")
+    c = dev.kv_cache(b, heads, 8, 64, wgf.F16)
+    c.append(give(wgf, dev, k, "f16"), give(wgf, dev, v, "f16"), counts=lens)
+    out = take(c.attention(give(wgf, dev, q, "f16")), "f16")
+    for i in [17, b - 1, *(int(n) for n in g.integers(0, b, 100))]:
+        kk, vv = (np.stack([ref.stands_for(x[i, h, : lens[i]]) for h in range(heads)]) for x in (k, v))
+        want, bound = ref.attention(q[i], kk, vv, 8 ** -0.5)
+        close(out[i], want, bound + ref.rounding(want, "f16"))
+
+
 # ---- 4-bit weights --------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("n,k,group", [(1, 1, 32), (16, 64, 64), (33, 70, 32), (50, 300, 128), (17, 200, 64), (40, 129, 128)])
@@ -534,6 +578,28 @@ def test_fused_append_is_the_operators_one_by_one(kind, dim, heads, kv_heads, wg
         at += t
     for a, b in zip(layers[0].cache.read(), layers[1].cache.read()):
         np.testing.assert_array_equal(a.as_slice(), b.as_slice())
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim", [8, 24, 72, 200, 248])
+def test_fused_append_of_uneven_heads(kind, dim, wgf, dev):
+    """Heads whose halves take no whole vector of the type, and operands that stand at odd places."""
+    g = seeded(24, dim + 1)
+    q, k, v = (draw(g, (2, h, 67, dim + 1), kind) for h in (3, 1, 1))
+    w, (cos, sin) = draw(g, (dim,), kind, 0.2, 1.0), tables(100, dim, kind)
+    tw, tc, ts = (give(wgf, dev, x, kind) for x in (w, cos, sin))
+    tq, tk, tv = (give(wgf, dev, x, kind).slice([(0, 2), (0, x.shape[1]), (0, 67), (1, dim + 1)]) for x in (q, k, v))
+    one, two = (dev.kv_cache(2, 1, dim, 100, code_of(wgf, kind)) for _ in range(2))
+    for c in (one, two):
+        c.append(tv.slice([(0, 2), (0, 1), (0, 5), (0, dim)]), tv.slice([(0, 2), (0, 1), (0, 5), (0, dim)]))
+    a = one.append_qk(tq, tk, tv, tw, tw, tc, ts, eps=1e-5)
+    b, kk = tq.qk_norm_rope(tk, tw, tw, tc, ts, eps=1e-5, start=5)
+    two.append(kk, tv)
+    np.testing.assert_array_equal(a.as_slice(), b.as_slice())
+    for x, y in zip(one.read(), two.read()):
+        np.testing.assert_array_equal(x.as_slice(), y.as_slice())
+    want, off = ref.norm_rope(q[..., 1:].reshape(6, 67, dim), w, cos, sin, 1e-5, 5 + np.arange(67))
+    close(take(a, kind).reshape(6, 67, dim), want, off * 1.01 + ref.rounding(want, kind) * 1.01)
 
 
 def test_fused_append_of_a_padded_batch(wgf, dev):
