@@ -20,8 +20,9 @@
 //     a CTA), and every CTA takes an equal stretch of it, as the kernel itself computes from the lengths: ragged
 //     batches are even, and a recorded launch stays even while its sequences grow.  The last CTA to finish a job
 //     that several have a stretch of joins their parts, in their order, so results do not depend on timing.
-// One token over 131071 of 8 kv heads, 269 MB: the CTAs' loops take 42 us (6.4 TB/s of the measured 6.56), a pass 56 us with
-// the launch, the first loads and the joining; with two half blocks in a ring instead of three it took 87.
+// One token over 131071 of 8 kv heads, 269 MB: the CTAs' loops take 42 us (6.4 TB/s of the measured 6.56), a pass 55 us with
+// the launch, the first loads and the joining; with two half blocks in a ring instead of three it took 87.  32 sequences of up to
+// 8192 tokens, 310 MB: 75 us, 84 where each job had a number of CTAs of its own.
 #include <algorithm>
 
 #include "decode.hpp"

@@ -382,6 +382,7 @@ Q4TcPlan q4_tc_plan(Device& dev, const Q4Weight& w, int64_t rows) {
 bool q4_tc_run(Device& dev, const Q4Weight& w, const Q4TcPlan& plan, const TensorData& x, int64_t rows, void* y) {
     const bool bf16 = x.dtype == DType::BF16;
     const int64_t stride = x.layout.strides[0];
+    if (rows >= (1ll << 31) - 256) return false;              // coordinates of TMA are 32 bits
     CUtensorMap map;
     if (!dev.dry && !encode_3d(&map, bf16, x.base_ptr(), w.k, rows, 1, stride, rows * stride, kBK, (unsigned)plan.tile_rows)) return false;
     Q4TcParams p{};
