@@ -476,6 +476,22 @@ def test_q4_product_on_tensor_cores_of_bad_values_and_views(wgf, dev):
     assert np.isfinite(np.asarray(take(back, "f16"))[:, keep]).all()
 
 
+@pytest.mark.parametrize("kind,rows,n,k", [("f16", 500, 11000, 3000), ("bf16", 33, 2000, 8200)])
+def test_q4_product_on_tensor_cores_in_shares(kind, rows, n, k, wgf, dev):
+    """Whole tiles, and behind them tiles whose columns are dealt out; the same bits each time, whoever is last."""
+    g = seeded(29, 3)
+    w, x = draw(g, (n, k), kind, 0.02), draw(g, (rows, k), kind)
+    c, s = ref.q4_quantize(w, 64, kind)
+    t, a = give(wgf, dev, w, kind).quantize_q4(64), give(wgf, dev, x, kind)
+    dev.set_timing(True)
+    out = a.mat_mul_q4(t)
+    got = take(out, kind)
+    assert "q4_tc" in out.timing_labels()
+    close(got, *ref.q4_product(x, ref.q4_values(c, s, 64), kind, through=kind))
+    for _ in range(10):
+        np.testing.assert_array_equal(take(a.mat_mul_q4(t), kind), got)
+
+
 def test_q4_product_on_tensor_cores_replayed(wgf, dev):
     g = seeded(29, 2)
     rows, n, k = 300, 1100, 1100

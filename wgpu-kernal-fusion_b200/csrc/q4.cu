@@ -721,9 +721,9 @@ static RowsPlan plan_rows(Device& dev, const Q4Weight& w, int64_t rows, int part
 
 // Which way rows take: in blocks through the kernel above, through the tensor cores (q4_tc.cu), or through weights that are
 // written out and the matrix product.  Rows of 16 bits: what each would take is estimated, in us.  Measured, blocks / tensor
-// cores / written out: 11008 x 4096, 40 rows 38 / 36 / 660 (the matrix product of fewer than 64 rows is strided), 64 rows 80 / 36 / 63,
-// 128 rows 118 / 39 / 63, 500 rows 380 / 73 / 80, 1000 rows 722 / 105 / 107, 2048 rows 1450 / 163 / 145; 4096 x 4096, 40 rows 24 / 36 / -,
-// 64 rows 39 / 36 / 42, 800 rows 283 / 46 / 45; 1024 x 1024, 64 rows 11 / 15 / 23, 500 rows 28 / 16 / 26.
+// cores / written out: 11008 x 4096, 64 rows 79 / 35 / 63, 128 rows 116 / 38 / 63, 500 rows 373 / 63 / 80, 2048 rows 1450 / 163 / 145;
+// 4096 x 4096, 20 rows 17 / 18 / 440 (the matrix product of fewer than 64 rows is strided), 64 rows 38 / 20 / 42, 500 rows 179 / 40 / 44;
+// 600 x 4000, 64 rows 12 / 16 / 37, 256 rows 27 / 20 / 38; 1024 x 1024, 64 rows 11 / 13 / 23, 500 rows 27 / 16 / 26.
 // Rows of f32 have no tensor-core form, and the FFMA product is slow for rows like these: 4096 x 4096: 500 rows 501 in blocks, 615
 // written out; 11008 x 4096: 500 rows 1308 / 1562.
 enum class Q4Way { BLOCKS, TENSOR, WRITTEN };

@@ -12,12 +12,14 @@
 //                halves in the other order, so that the lanes of a store fall on different banks.
 //   warp 22      brings the codes and scales of two steps at a time by bulk copies
 // Every wait is bounded and reports through the device's error word.
-// 500 rows of f16 through 11008 x 4096: 67 us in two waves of tiles of 176 rows, where weights written out and the matrix product take
-// 76 together, and the products alone 27 at the measured rate of the tensor cores; 100 rows 35 us against 58.  A step of 64
-// columns takes 0.4 us with few rows of x and 0.5 with 256, while its products take 0.05 to 0.39: turning the codes into the operand, the
-// copies and the handing over of a step cost about 0.2 us each and overlap only in part (without the first 0.33, without all of them
-// 0.2), and with 256 rows L2 delivers x at about 9 TB/s.  Tried and not kept: 256 rows of weights a tile (half the traffic of x, one wave
-// of 500 rows: 74 us), two steps to a stage (72), two CTAs a SM with half the decoders (69), one lane that waits for its warp (115).
+// What the tiles leave of the last wave is filled by dividing its tiles along the columns: a CTA then leaves its f32 sums in memory, and
+// the last of a tile's CTAs adds them up in their order.  64 rows of bf16 through 4096 x 4096: 17 us, 34 undivided; through 4096 x
+// 11008: 29, 78 undivided; 500 rows of f16 through 11008 x 4096: 60, 67 undivided (whole tiles alone, of 176 rows), where weights
+// written out and the matrix product take 76 together, and the products alone 27 at the measured rate of the tensor cores.
+// A step of 64 columns takes 0.4 us with few rows of x and 0.5 with 256, while its products take 0.05 to 0.39: turning the codes into the
+// operand, the copies and the handing over of a step cost about 0.2 us each and overlap only in part (without the first 0.33, without
+// all of them 0.2), and with 256 rows L2 delivers x at about 9 TB/s.  Tried and not kept (500 rows): 256 rows of weights a tile (half the
+// traffic of x: 74 us), two steps to a stage (72), two CTAs a SM with half the decoders (69), one lane that waits for its warp (115).
 #include <algorithm>
 #include <type_traits>
 
@@ -52,8 +54,26 @@ struct Q4TcParams {
     DType scale_dtype;
     int tile_rows;                       // of x
     int tiles_m, tiles_n, stages;
+    int whole, shares, share_chunks;     // tiles of one unit each; units of each of the others, and their steps (an even number)
+    float* part;                         // sums of those units: [unit][row of x][128]
+    unsigned* tickets;                   // of those tiles
     int scale_bytes, tile_bytes;         // of a scale; of a tile of 16 rows in a pair of steps
     unsigned* error;
+};
+
+// A unit of work: a tile, or a share of its steps
+struct Unit {
+    int tile, share, begin, end;         // share < 0: all of it
+    __device__ __forceinline__ Unit(const Q4TcParams& p, int u) {
+        tile = u, share = -1, begin = 0, end = p.chunks;
+        if (u >= p.whole) {
+            tile = p.whole + (u - p.whole) / p.shares;
+            share = (u - p.whole) % p.shares;
+            begin = share * p.share_chunks;
+            end = min(end, begin + p.share_chunks);
+            if (p.shares == 1) share = -1;
+        }
+    }
 };
 
 // fp32 accumulator, both operands K-major f16 or bf16, M = 128, N = rows
@@ -163,7 +183,7 @@ template <typename T, bool SAME, bool G32>
 __global__ void __launch_bounds__(kThreadsTc, 1) q4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ Q4TcParams p) {
     extern __shared__ unsigned char smem_raw[];
     __shared__ alignas(8) unsigned long long bars[3 * kMaxStages + 4 + 2 * kPairs];
-    __shared__ unsigned tmem_slot;
+    __shared__ unsigned tmem_slot, last;
     const unsigned stages_at = (smem_u32(smem_raw) + 1023) & ~1023u;          // the swizzle wants 1024-byte alignment
     const unsigned stage_bytes = kWBytes + (unsigned)p.tile_rows * kBK * 2;
     const unsigned pairs_at = stages_at + p.stages * stage_bytes, pair_bytes = 8u * p.tile_bytes;
@@ -197,16 +217,17 @@ __global__ void __launch_bounds__(kThreadsTc, 1) q4_tc_kernel(const __grid_const
     __syncthreads();
     tc_fence_after();
     const unsigned tmem = tmem_slot;
-    const int tiles = p.tiles_m * p.tiles_n;
+    const int units = p.whole + (p.tiles_m * p.tiles_n - p.whole) * p.shares;
 
     if (warp == 0) {
         if (lane == 0) {
             int stage = 0;
             unsigned phase = 1;                       // a fresh barrier counts as released
             bool ok = true;
-            for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
-                const int m0 = tile % p.tiles_m * p.tile_rows;
-                for (int kb = 0; kb < p.chunks; ++kb) {
+            for (int i = blockIdx.x; i < units && ok; i += gridDim.x) {
+                const Unit u(p, i);
+                const int m0 = u.tile % p.tiles_m * p.tile_rows;
+                for (int kb = u.begin; kb < u.end; ++kb) {
                     if (!mbar_wait(empty(stage), phase)) {
                         atomicExch(p.error, 11u);
                         ok = false;
@@ -225,13 +246,14 @@ __global__ void __launch_bounds__(kThreadsTc, 1) q4_tc_kernel(const __grid_const
             int stage = 0, acc = 0;
             unsigned phase = 0, acc_phase = 1;
             bool ok = true;
-            for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+            for (int n = blockIdx.x; n < units && ok; n += gridDim.x) {
+                const Unit u(p, n);
                 if (!mbar_wait(acc_empty(acc), acc_phase)) {
                     atomicExch(p.error, 12u);
                     break;
                 }
                 tc_fence_after();
-                for (int kb = 0; kb < p.chunks; ++kb) {
+                for (int kb = u.begin; kb < u.end; ++kb) {
                     if (!mbar_wait(x_full(stage), phase) || !mbar_wait(w_full(stage), phase)) {
                         atomicExch(p.error, 13u);
                         ok = false;
@@ -240,7 +262,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) q4_tc_kernel(const __grid_const
                     tc_fence_after();
                     const unsigned long long w = first + (unsigned)stage * (stage_bytes >> 4), x = w + (kWBytes >> 4);
 #pragma unroll
-                    for (int i = 0; i < kBK / 16; ++i) umma_f16(tmem + (unsigned)acc * 256, w + 2 * i, x + 2 * i, idesc, (kb | i) != 0);
+                    for (int i = 0; i < kBK / 16; ++i) umma_f16(tmem + (unsigned)acc * 256, w + 2 * i, x + 2 * i, idesc, kb != u.begin || i != 0);
                     umma_commit(empty(stage));
                     if (++stage == p.stages) stage = 0, phase ^= 1;
                 }
@@ -252,21 +274,26 @@ __global__ void __launch_bounds__(kThreadsTc, 1) q4_tc_kernel(const __grid_const
         const int quarter = warp & 3;                 // of the accumulator's lanes
         int acc = 0;
         unsigned acc_phase = 0;
-        for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+        for (int i = blockIdx.x; i < units; i += gridDim.x) {
+            const Unit u(p, i);
             if (!mbar_wait(acc_full(acc), acc_phase)) {
                 if (lane == 0) atomicExch(p.error, 14u);
                 break;
             }
             tc_fence_after();
-            const long long m0 = (long long)(tile % p.tiles_m) * p.tile_rows;
+            const long long m0 = (long long)(u.tile % p.tiles_m) * p.tile_rows, n = (long long)(u.tile / p.tiles_m) * 128 + quarter * 32 + lane;
             const int live = (int)min((long long)p.tile_rows, p.rows - m0);
-            const long long n = (long long)(tile / p.tiles_m) * 128 + quarter * 32 + lane;
             T* to = (T*)p.y + m0 * p.n + n;
+            float* mine = u.share < 0 ? nullptr : p.part + (long long)(i - p.whole) * p.tile_rows * 128 + quarter * 32 + lane;
             for (int c = 0; c < live; c += 32) {
                 unsigned v[32];
                 tmem_ld_32x32(tmem + ((unsigned)(quarter * 32) << 16) + (unsigned)(acc * 256 + c), v);
                 tmem_ld_wait();
-                if (n < p.n) {
+                if (mine) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if (c + j < live) mine[(c + j) * 128] = __uint_as_float(v[j]);
+                } else if (n < p.n) {
 #pragma unroll
                     for (int j = 0; j < 32; ++j)
                         if (c + j < live) to[(c + j) * p.n] = decode::from_f<T>(__uint_as_float(v[j]));
@@ -288,12 +315,13 @@ __global__ void __launch_bounds__(kThreadsTc, 1) q4_tc_kernel(const __grid_const
         int stage = 0, buffer = 0;
         unsigned phase = 1, pair_phase = 0;
         bool ok = true;
-        for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x)
-            for (int kb = 0; kb < p.chunks; kb += 2) {
+        for (int i = blockIdx.x; i < units && ok; i += gridDim.x) {
+            const Unit work(p, i);
+            for (int kb = work.begin; kb < work.end; kb += 2) {
                 int s = stage + odd;
                 unsigned s_phase = phase;
                 if (s >= p.stages) s -= p.stages, s_phase ^= 1;
-                const bool live = kb + odd < p.chunks;
+                const bool live = kb + odd < work.end;
                 if (!mbar_wait(pair_full(buffer), pair_phase) || (live && !mbar_wait(empty(s), s_phase))) {
                     if (lane == 0) atomicExch(p.error, 15u);
                     ok = false;
@@ -323,27 +351,29 @@ __global__ void __launch_bounds__(kThreadsTc, 1) q4_tc_kernel(const __grid_const
                     if (live) mbar_arrive(w_full(s));
                     mbar_arrive(pair_empty(buffer));
                 }
-                stage += min(2, p.chunks - kb);
+                stage += min(2, work.end - kb);
                 if (stage >= p.stages) stage -= p.stages, phase ^= 1;
                 if (++buffer == kPairs) buffer = 0, pair_phase ^= 1;
             }
+        }
     } else {
         int buffer = 0;
         unsigned phase = 1;
         bool ok = true;
-        for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+        for (int i = blockIdx.x; i < units && ok; i += gridDim.x) {
+            const Unit u(p, i);
             // tiles behind the last are the last again: nobody reads what becomes of their rows
-            const long long rt = min(tile / p.tiles_m * 8 + (lane & 7), p.row_tiles - 1);
+            const long long rt = min(u.tile / p.tiles_m * 8 + (lane & 7), p.row_tiles - 1);
             const uint4* words = p.codes + rt * p.chunks * 32;
             const unsigned char* scales = (const unsigned char*)p.scales + rt * p.groups * 16 * p.scale_bytes;
-            for (int kb = 0; kb < p.chunks; kb += 2) {
+            for (int kb = u.begin; kb < u.end; kb += 2) {
                 if (!mbar_wait(pair_empty(buffer), phase)) {
                     if (lane == 0) atomicExch(p.error, 16u);
                     ok = false;
                     break;
                 }
                 const int q = kb * 64 >> p.group_log2;
-                const unsigned wb = min(2, p.chunks - kb) * 512u, sb = min(128 >> p.group_log2, p.groups - q) * 16u * p.scale_bytes;
+                const unsigned wb = min(2, u.end - kb) * 512u, sb = min(128 >> p.group_log2, p.groups - q) * 16u * p.scale_bytes;
                 if (lane == 0) mbar_expect_tx(pair_full(buffer), 8 * (wb + sb));
                 __syncwarp();
                 if (lane < 8) {
@@ -361,20 +391,56 @@ __global__ void __launch_bounds__(kThreadsTc, 1) q4_tc_kernel(const __grid_const
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
+    // A CTA has at most one share of a tile, its last unit.  The last CTA of a tile's adds up what all have left, in their order.
+    if (p.shares == 1) return;
+    const int i = blockIdx.x + (units - 1 - blockIdx.x) / gridDim.x * gridDim.x;
+    if (i < p.whole) return;
+    const Unit u(p, i);
+    if (threadIdx.x == 0) {
+        __threadfence();                                       // behind the barrier: for all that the CTA has written
+        last = atomicAdd(p.tickets + (u.tile - p.whole), 1u) == (unsigned)p.shares - 1;
+        __threadfence();
+    }
+    __syncthreads();
+    if (!last) return;
+    const long long m0 = (long long)(u.tile % p.tiles_m) * p.tile_rows, n0 = (long long)(u.tile / p.tiles_m) * 128 + lane * 4;
+    const int live = (int)min((long long)p.tile_rows, p.rows - m0);
+    const float* parts = p.part + (long long)(u.tile - p.whole) * p.shares * p.tile_rows * 128 + lane * 4;
+    for (int c = warp; c < live; c += kThreadsTc / 32) {       // a warp has whole rows of x
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+        for (int s = 0; s < p.shares; ++s) {
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(parts + ((long long)s * p.tile_rows + c) * 128));
+            sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+        }
+        const float f[4] = {sum.x, sum.y, sum.z, sum.w};
+        T* row = (T*)p.y + (m0 + c) * p.n + n0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (n0 + e < p.n) row[e] = decode::from_f<T>(f[e]);
+    }
+    if (threadIdx.x == 0) p.tickets[u.tile - p.whole] = 0;
 }
 
 }  // namespace
 
 // Tiles of few rows of x cost nearly what tiles of many do, as the time goes into the weights' side: so as few waves as 256 rows
-// allow, and of those the smallest tiles.  In us: a step of 64 columns takes 0.44 with 64 rows of x, 0.47 with 128, 0.55 with 256.
+// allow.  The tiles of the last wave are divided along the columns, where the SMs that they leave would wait, if the adding up
+// costs less.  In us: a step of 64 columns takes 0.44 with 64 rows of x, 0.47 with 128, 0.55 with 256; adding up 2.5, and 0.0105 for
+// each row of x in each share.
 Q4TcPlan q4_tc_plan(Device& dev, const Q4Weight& w, int64_t rows) {
     Q4TcPlan best;
-    const int64_t tiles_n = (w.row_tiles + 7) / 8, least = (rows + 255) / 256;
+    const int64_t tiles_n = (w.row_tiles + 7) / 8, least = (rows + 255) / 256, sms = dev.sm_count;
     for (int64_t t = least; t < least + 16; ++t) {
-        const int64_t tile_rows = ((rows + t - 1) / t + 15) / 16 * 16;
-        const int64_t waves = (tiles_n * t + dev.sm_count - 1) / dev.sm_count;
-        const double us = 5.0 + (double)waves * (double)w.chunks * (0.40 + 0.0006 * (double)tile_rows);
-        if (us < best.us) best = {(int)tile_rows, us};
+        const int64_t tile_rows = ((rows + t - 1) / t + 15) / 16 * 16, tiles = tiles_n * ((rows + tile_rows - 1) / tile_rows), whole = tiles / sms * sms;
+        const double step = 0.40 + 0.0006 * (double)tile_rows;
+        for (int64_t s = 1; s <= 32; ++s) {
+            const int64_t steps = s == 1 ? w.chunks : ((w.chunks + s - 1) / s + 1) / 2 * 2, shares = (w.chunks + steps - 1) / steps;
+            if (s > 1 && (shares < s || whole == tiles || (tiles - whole) * shares > sms)) continue;      // a CTA has one share at most
+            const double us = 5.0 + ((double)(whole / sms * w.chunks) + (tiles > whole ? (double)steps : 0)) * step +
+                              (shares > 1 ? 2.5 + 0.0105 * (double)(shares * tile_rows) : 0);
+            if (us < best.us) best = {(int)tile_rows, (int)whole, (int)shares, (int)steps, us};
+        }
     }
     return best;
 }
@@ -405,7 +471,17 @@ bool q4_tc_run(Device& dev, const Q4Weight& w, const Q4TcPlan& plan, const Tenso
     const int stage_bytes = kWBytes + plan.tile_rows * kBK * 2, pairs_bytes = kPairs * 8 * p.tile_bytes;
     p.stages = std::min(kMaxStages, (kRoom - pairs_bytes) / stage_bytes);
     p.error = dev.error_word();
-    const unsigned grid = (unsigned)std::min<int64_t>((int64_t)p.tiles_m * p.tiles_n, dev.sm_count);
+    p.whole = plan.whole;
+    p.shares = plan.shares;
+    p.share_chunks = plan.share_chunks;
+    const int64_t divided = (int64_t)p.tiles_m * p.tiles_n - p.whole;     // fewer than SMs
+    BufferRef scratch;
+    if (p.shares > 1) {
+        scratch = dev.alloc((size_t)(divided * p.shares * p.tile_rows) * 128 * sizeof(float), false);
+        p.part = (float*)scratch->ptr;
+        p.tickets = (unsigned*)dev.counters();
+    }
+    const unsigned grid = (unsigned)std::min<int64_t>(p.whole + divided * p.shares, dev.sm_count);
     const int smem = p.stages * stage_bytes + pairs_bytes + 1024;
     dev.begin_launch("q4_tc");
     if (!dev.dry) {

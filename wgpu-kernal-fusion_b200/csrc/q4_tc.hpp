@@ -6,6 +6,8 @@ namespace wgf {
 
 struct Q4TcPlan {
     int tile_rows = 0;                 // rows of x of a tile
+    int whole = 0;                     // tiles that one CTA does from end to end; the others are done in
+    int shares = 1, share_chunks = 0;  // shares of so many steps
     double us = 1e300;                 // about what it takes
 };
 Q4TcPlan q4_tc_plan(Device& dev, const Q4Weight& w, int64_t rows);
