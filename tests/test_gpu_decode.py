@@ -492,6 +492,17 @@ def test_q4_product_on_tensor_cores_in_shares(kind, rows, n, k, wgf, dev):
         np.testing.assert_array_equal(take(a.mat_mul_q4(t), kind), got)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+def test_q4_product_of_very_long_rows(kind, wgf, dev):
+    """A row of x is more than the shared memory of eight SMs."""
+    g = seeded(29, 4)
+    rows, n, k = 3, 20, 700_040
+    w, x = draw(g, (n, k), kind, 0.02), draw(g, (rows, k), kind)
+    c, s = ref.q4_quantize(w, 128, kind)
+    out = give(wgf, dev, x, kind).mat_mul_q4(give(wgf, dev, w, kind).quantize_q4(128))
+    close(take(out, kind), *ref.q4_product(x, ref.q4_values(c, s, 128), kind, through=kind))
+
+
 def test_q4_product_on_tensor_cores_replayed(wgf, dev):
     g = seeded(29, 2)
     rows, n, k = 300, 1100, 1100

@@ -756,7 +756,8 @@ TensorData run_matmul_q4(Device& dev, const TensorData& x_in, const Q4Weight& w)
     dev.wait_for(*x.buf);
     const int parts = x.dtype == DType::F32 ? 3 : 1;
     const RowsPlan plan = plan_rows(dev, w, rows, parts);
-    const Q4TcPlan tc = q4_tc_plan(dev, w, rows);
+    // (rows that one block holds are read off the codes once: nothing is faster)
+    const Q4TcPlan tc = parts == 1 && (rows > 8 || !plan.shares) ? q4_tc_plan(dev, w, rows) : Q4TcPlan();
     const Q4Way way = choose_way(dev, plan, tc, w, rows, parts);
     dev.note_recorded_buffer(w.codes);
     dev.note_recorded_buffer(w.scales);

@@ -431,15 +431,19 @@ __global__ void __launch_bounds__(kThreadsTc, 1) q4_tc_kernel(const __grid_const
 Q4TcPlan q4_tc_plan(Device& dev, const Q4Weight& w, int64_t rows) {
     Q4TcPlan best;
     const int64_t tiles_n = (w.row_tiles + 7) / 8, least = (rows + 255) / 256, sms = dev.sm_count;
-    for (int64_t t = least; t < least + 16; ++t) {
-        const int64_t tile_rows = ((rows + t - 1) / t + 15) / 16 * 16, tiles = tiles_n * ((rows + tile_rows - 1) / tile_rows), whole = tiles / sms * sms;
-        const double step = 0.40 + 0.0006 * (double)tile_rows;
-        for (int64_t s = 1; s <= 32; ++s) {
-            const int64_t steps = s == 1 ? w.chunks : ((w.chunks + s - 1) / s + 1) / 2 * 2, shares = (w.chunks + steps - 1) / steps;
-            if (s > 1 && (shares < s || whole == tiles || (tiles - whole) * shares > sms)) continue;      // a CTA has one share at most
-            const double us = 5.0 + ((double)(whole / sms * w.chunks) + (tiles > whole ? (double)steps : 0)) * step +
-                              (shares > 1 ? 2.5 + 0.0105 * (double)(shares * tile_rows) : 0);
-            if (us < best.us) best = {(int)tile_rows, (int)whole, (int)shares, (int)steps, us};
+    int64_t before = 0;
+    for (int64_t t = least; t < least + 8; ++t) {
+        const int64_t tile_rows = ((rows + t - 1) / t + 15) / 16 * 16;
+        if (tile_rows == before) continue;
+        before = tile_rows;
+        const int64_t tiles = tiles_n * ((rows + tile_rows - 1) / tile_rows), whole = tiles / sms * sms, rest = tiles - whole;
+        const double step = 0.40 + 0.0006 * (double)tile_rows, start = 5.0 + (double)(whole / sms * w.chunks) * step;
+        const int most = rest ? (int)std::min<int64_t>(sms / rest, 32) : 1;      // a CTA has one share at most
+        for (int s = 1; s <= most; ++s) {
+            const int steps = s == 1 ? (int)w.chunks : (((int)w.chunks + s - 1) / s + 1) / 2 * 2, shares = ((int)w.chunks + steps - 1) / steps;
+            if (shares < s) continue;
+            const double us = start + (rest ? (double)steps * step : 0) + (shares > 1 ? 2.5 + 0.0105 * (double)(shares * tile_rows) : 0);
+            if (us < best.us) best = {(int)tile_rows, (int)whole, shares, steps, us};
         }
     }
     return best;
