@@ -14,7 +14,7 @@
 // Every wait is bounded and reports through the device's error word.
 // What the tiles leave of the last wave is filled by dividing its tiles along the columns: a CTA then leaves its f32 sums in memory, and
 // the last of a tile's CTAs adds them up in their order.  64 rows of bf16 through 4096 x 4096: 17 us, 34 undivided; through 4096 x
-// 11008: 29, 78 undivided; 500 rows of f16 through 11008 x 4096: 60, 67 undivided (whole tiles alone, of 176 rows), where weights
+// 11008: 29, 78 undivided; 500 rows of f16 through 11008 x 4096: 62, 67 undivided (whole tiles alone, of 176 rows), where weights
 // written out and the matrix product take 76 together, and the products alone 27 at the measured rate of the tensor cores.
 // A step of 64 columns takes 0.4 us with few rows of x and 0.5 with 256, while its products take 0.05 to 0.39: turning the codes into the
 // operand, the copies and the handing over of a step cost about 0.2 us each and overlap only in part (without the first 0.33, without
@@ -80,6 +80,9 @@ struct Unit {
 __device__ __forceinline__ unsigned instruction(bool bf16, int rows) {
     return (1u << 4) | (bf16 ? 1u << 7 | 1u << 10 : 0u) | (unsigned)(rows >> 3) << 17 | (128u >> 4) << 24;
 }
+
+// Lanes that give up on a wait take the others of their warp along.
+__device__ __forceinline__ bool all_of_warp(bool ok) { return __all_sync(0xffffffffu, ok); }
 
 // What a lane needs of a tile of 16 rows by 64 columns: its words, and as they are stored the scales of rows g and g + 8 for
 // each group.  SAME: scales of the type of x, two in a word.
@@ -229,7 +232,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) q4_tc_kernel(const __grid_const
                 const int m0 = u.tile % p.tiles_m * p.tile_rows;
                 for (int kb = u.begin; kb < u.end; ++kb) {
                     if (!mbar_wait(empty(stage), phase)) {
-                        atomicExch(p.error, 11u);
+                        atomicExch(p.error, 81u);
                         ok = false;
                         break;
                     }
@@ -238,6 +241,8 @@ __global__ void __launch_bounds__(kThreadsTc, 1) q4_tc_kernel(const __grid_const
                     if (++stage == p.stages) stage = 0, phase ^= 1;
                 }
             }
+            if (!ok)                                  // what is on its way lands before the CTA ends
+                for (int s = 0; s < p.stages; ++s) mbar_wait(x_full(s), s < stage ? phase ^ 1 : phase);
         }
     } else if (warp == 1) {
         if (lane == 0) {
@@ -249,13 +254,13 @@ __global__ void __launch_bounds__(kThreadsTc, 1) q4_tc_kernel(const __grid_const
             for (int n = blockIdx.x; n < units && ok; n += gridDim.x) {
                 const Unit u(p, n);
                 if (!mbar_wait(acc_empty(acc), acc_phase)) {
-                    atomicExch(p.error, 12u);
+                    atomicExch(p.error, 82u);
                     break;
                 }
                 tc_fence_after();
                 for (int kb = u.begin; kb < u.end; ++kb) {
                     if (!mbar_wait(x_full(stage), phase) || !mbar_wait(w_full(stage), phase)) {
-                        atomicExch(p.error, 13u);
+                        atomicExch(p.error, 83u);
                         ok = false;
                         break;
                     }
@@ -276,8 +281,8 @@ __global__ void __launch_bounds__(kThreadsTc, 1) q4_tc_kernel(const __grid_const
         unsigned acc_phase = 0;
         for (int i = blockIdx.x; i < units; i += gridDim.x) {
             const Unit u(p, i);
-            if (!mbar_wait(acc_full(acc), acc_phase)) {
-                if (lane == 0) atomicExch(p.error, 14u);
+            if (!all_of_warp(mbar_wait(acc_full(acc), acc_phase))) {
+                if (lane == 0) atomicExch(p.error, 84u);
                 break;
             }
             tc_fence_after();
@@ -322,8 +327,8 @@ __global__ void __launch_bounds__(kThreadsTc, 1) q4_tc_kernel(const __grid_const
                 unsigned s_phase = phase;
                 if (s >= p.stages) s -= p.stages, s_phase ^= 1;
                 const bool live = kb + odd < work.end;
-                if (!mbar_wait(pair_full(buffer), pair_phase) || (live && !mbar_wait(empty(s), s_phase))) {
-                    if (lane == 0) atomicExch(p.error, 15u);
+                if (!all_of_warp(mbar_wait(pair_full(buffer), pair_phase) && (!live || mbar_wait(empty(s), s_phase)))) {
+                    if (lane == 0) atomicExch(p.error, 85u);
                     ok = false;
                     break;
                 }
@@ -367,8 +372,8 @@ __global__ void __launch_bounds__(kThreadsTc, 1) q4_tc_kernel(const __grid_const
             const uint4* words = p.codes + rt * p.chunks * 32;
             const unsigned char* scales = (const unsigned char*)p.scales + rt * p.groups * 16 * p.scale_bytes;
             for (int kb = u.begin; kb < u.end; kb += 2) {
-                if (!mbar_wait(pair_empty(buffer), phase)) {
-                    if (lane == 0) atomicExch(p.error, 16u);
+                if (!all_of_warp(mbar_wait(pair_empty(buffer), phase))) {
+                    if (lane == 0) atomicExch(p.error, 86u);
                     ok = false;
                     break;
                 }
@@ -384,6 +389,8 @@ __global__ void __launch_bounds__(kThreadsTc, 1) q4_tc_kernel(const __grid_const
                 if (++buffer == kPairs) buffer = 0, phase ^= 1;
             }
         }
+        if (!ok)
+            for (int b = 0; b < kPairs; ++b) mbar_wait(pair_full(b), b < buffer ? phase ^ 1 : phase);
     }
     tc_fence_before();
     __syncthreads();
