@@ -417,9 +417,9 @@ def test_q4_product(kind, rows, n, k, group, wgf, dev):
 
 
 @pytest.mark.parametrize("kind", KINDS)
-@pytest.mark.parametrize("rows,n,k,group,way", [(700, 72, 64, 32, {"f32": "q4_dequantize"}), (3001, 130, 70, 32, {"f32": "q4_dequantize"}), (200, 40, 300, 128, {}), (65, 300, 1100, 64, {}),
-                                                (600, 1500, 2100, 64, {"f32": "q4_dequantize", "f16": "q4_tc", "bf16": "q4_tc"}),
-                                                (2300, 3400, 260, 64, {"f32": "q4_dequantize"})])
+@pytest.mark.parametrize("rows,n,k,group,way", [(700, 72, 64, 32, {}), (3001, 130, 70, 32, {}), (200, 40, 300, 128, {}), (65, 300, 1100, 64, {}),
+                                                (600, 1500, 2100, 64, {"f32": "q4_tc", "f16": "q4_tc", "bf16": "q4_tc"}),
+                                                (2300, 3400, 260, 64, {"f32": "q4_tc"})])
 def test_q4_product_of_many_rows(kind, rows, n, k, group, way, wgf, dev):
     """Rows in blocks, on the tensor cores, and weights that are written out for the matrix product, in padded rows where k is odd for it."""
     g = seeded(23, rows)
@@ -448,6 +448,24 @@ def test_q4_product_on_tensor_cores(kind, scale_kind, group, rows, n, k, wgf, de
     out = give(wgf, dev, x, kind).mat_mul_q4(t)
     close(take(out, kind), *ref.q4_product(x, ref.q4_values(c, s, group), kind, through=kind))
     assert "q4_tc" in out.timing_labels()
+
+
+@pytest.mark.parametrize("scale_kind", KINDS)
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("rows,n,k", [(300, 1100, 1100), (257, 1030, 1091), (161, 2200, 1985), (97, 4000, 2113)])
+def test_q4_product_of_f32_on_tensor_cores(scale_kind, group, rows, n, k, wgf, dev):
+    """Rows of f32 keep their digits: codes and parts are exact, and only sums round."""
+    g = seeded(30, rows + n + k + group)
+    w, x = draw(g, (n, k), scale_kind, 0.02), draw(g, (rows, k + 1), "f32")
+    x[5] *= 1e30
+    x[6] *= 1e-25
+    c, s = ref.q4_quantize(w, group, scale_kind)
+    t = give(wgf, dev, w, scale_kind).quantize_q4(group)
+    dev.set_timing(True)
+    out = give(wgf, dev, x, "f32").slice([(0, rows), (1, k + 1)]).mat_mul_q4(t)
+    got = out.as_slice()
+    assert "q4_tc" in out.timing_labels()
+    close(got, *ref.q4_product(x[:, 1:], ref.q4_values(c, s, group), "f32"))
 
 
 def test_q4_product_on_tensor_cores_of_bad_values_and_views(wgf, dev):

@@ -227,6 +227,19 @@ template <typename T> __device__ __forceinline__ void operands(const T* row, lon
         out[q] = make_uint4(h[q][0] | (unsigned)h[q][1] << 16, h[q][2] | (unsigned)h[q][3] << 16, h[q][4] | (unsigned)h[q][5] << 16, h[q][6] | (unsigned)h[q][7] << 16);
 }
 
+// Rows of f32 as their parts, for the tensor cores: [rows / 32][part][32][stride]
+__global__ void q4_split_kernel(const float* __restrict__ x, long long x_stride, long long rows, long long k, __nv_bfloat16* __restrict__ out, long long stride) {
+    const long long pieces = stride / 8, total = rows * pieces;
+    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
+        const long long row = i / pieces, at = (i - row * pieces) * 8;
+        uint4 part[3];
+        operands<float>(x + row * x_stride, at, k, part);
+        __nv_bfloat16* to = out + (row / kExactRows * 3 * kExactRows + row % kExactRows) * stride + at;
+#pragma unroll
+        for (int q = 0; q < 3; ++q) *reinterpret_cast<uint4*>(to + q * kExactRows * stride) = part[q];
+    }
+}
+
 // The scales of rows g and g + 8, from what a lane's copy brought
 template <bool WIDE> __device__ __forceinline__ float2 two_scales(unsigned at, bool half) {
     if constexpr (WIDE) return shared_float2(at);
@@ -724,12 +737,12 @@ static RowsPlan plan_rows(Device& dev, const Q4Weight& w, int64_t rows, int part
 // cores / written out: 11008 x 4096, 64 rows 79 / 35 / 63, 128 rows 116 / 38 / 63, 500 rows 373 / 63 / 80, 2048 rows 1450 / 163 / 145;
 // 4096 x 4096, 20 rows 17 / 18 / 440 (the matrix product of fewer than 64 rows is strided), 64 rows 38 / 20 / 42, 500 rows 179 / 40 / 44;
 // 600 x 4000, 64 rows 12 / 16 / 37, 256 rows 27 / 20 / 38; 1024 x 1024, 64 rows 11 / 13 / 23, 500 rows 27 / 16 / 26.
-// Rows of f32 have no tensor-core form, and the FFMA product is slow for rows like these: 4096 x 4096: 500 rows 501 in blocks, 615
-// written out; 11008 x 4096: 500 rows 1308 / 1562.
+// Rows of f32, blocks / tensor cores (as three parts of bf16 each, with the taking apart) / written out for the FFMA product:
+// 4096 x 4096, 500 rows 501 / 138 / 615; 11008 x 4096, 500 rows 1308 / 328 / 1562.
 enum class Q4Way { BLOCKS, TENSOR, WRITTEN };
 static Q4Way choose_way(Device& dev, const RowsPlan& plan, const Q4TcPlan& tc, const Q4Weight& w, int64_t rows, int parts) {
-    if (parts > 1) return plan.shares && rows <= 512 ? Q4Way::BLOCKS : Q4Way::WRITTEN;
     const double blocks = plan.shares ? 3.0 + 0.021 * plan.cost : 1e30;
+    if (parts > 1) return blocks <= tc.us + 4.0 ? Q4Way::BLOCKS : Q4Way::TENSOR;      // 4: taking x apart
     // the matrix product: tiles of 256 x 256 for a pair of SMs, of which half a wave can be cut smaller
     const double tiles = (double)((rows + 255) / 256) * (double)((w.n + 255) / 256), waves = std::max(1.0, std::ceil(2.0 * tiles / (dev.sm_count / 2)) / 2);
     const double written = rows < 64 ? 1e30 : 3.0 + 0.55e-6 * (double)w.n * (double)w.k + 8.0 + 0.43 * waves * (double)w.chunks;
@@ -757,10 +770,21 @@ TensorData run_matmul_q4(Device& dev, const TensorData& x_in, const Q4Weight& w)
     const int parts = x.dtype == DType::F32 ? 3 : 1;
     const RowsPlan plan = plan_rows(dev, w, rows, parts);
     // (rows that one block holds are read off the codes once: nothing is faster)
-    const Q4TcPlan tc = parts == 1 && (rows > 8 || !plan.shares) ? q4_tc_plan(dev, w, rows) : Q4TcPlan();
+    const Q4TcPlan tc = rows > 8 || !plan.shares ? q4_tc_plan(dev, w, rows, parts > 1) : Q4TcPlan();
     const Q4Way way = choose_way(dev, plan, tc, w, rows, parts);
     dev.note_recorded_buffer(w.codes);
     dev.note_recorded_buffer(w.scales);
+    if (way == Q4Way::TENSOR && parts > 1) {
+        if (x.layout.strides[1] != 1 && w.k > 1) x = run_compact(dev, x);
+        const int64_t kp = (w.k + 7) / 8 * 8, tiles = (rows + kExactRows - 1) / kExactRows;
+        BufferRef split = dev.alloc((size_t)(tiles * 3 * kExactRows * kp) * 2, false);
+        out.buf = dev.alloc((size_t)(rows * w.n) * sizeof(float), false);
+        dev.begin_launch("q4_split");
+        if (!dev.dry)
+            q4_split_kernel<<<grid_for(dev, rows * kp / 8), 256, 0, dev.stream>>>((const float*)x.base_ptr(), x.layout.strides[0], rows, w.k, (__nv_bfloat16*)split->ptr, kp);
+        dev.end_launch();
+        if (q4_tc_run(dev, w, tc, split->ptr, DType::BF16, kp, rows, true, out.buf->ptr)) return out;
+    }
     if (way != Q4Way::BLOCKS) {
         // rows that begin at 16-byte borders, which the tensor-core kernels want
         const int64_t kp = parts == 1 ? (w.k + 7) / 8 * 8 : w.k;
@@ -774,9 +798,9 @@ TensorData run_matmul_q4(Device& dev, const TensorData& x_in, const Q4Weight& w)
             run_copy(dev, window, x);
             x = wide;
         }
-        if (way == Q4Way::TENSOR) {
+        if (way == Q4Way::TENSOR && parts == 1) {
             out.buf = dev.alloc((size_t)(rows * w.n) * dtype_size(x.dtype), false);
-            if (q4_tc_run(dev, w, tc, x, rows, out.base_ptr())) return out;
+            if (q4_tc_run(dev, w, tc, x.base_ptr(), x.dtype, x.layout.strides[0], rows, false, out.base_ptr())) return out;
         }
         x.layout.shape = {rows, kp};
         TensorData full = dequantize_rows(dev, w, x.dtype, kp);

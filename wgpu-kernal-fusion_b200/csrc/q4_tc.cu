@@ -1,4 +1,4 @@
-// Products with 4-bit weights for many rows of f16 or bf16, on the tensor cores.
+// Products with 4-bit weights for many rows, on the tensor cores.
 //
 //   y[m, n] = sum_k x[m, k] w[n, k],   w[n, k] = scale[n, k / group] * (code[n, k] - 8), rounded once to the type of x
 //
@@ -12,6 +12,11 @@
 //                halves in the other order, so that the lanes of a store fall on different banks.
 //   warp 22      brings the codes and scales of two steps at a time by bulk copies
 // Every wait is bounded and reports through the device's error word.
+//
+// Rows of f32 (EXACT): 32 rows of x are three times 32 rows of bf16 parts, which together have their 24 bits; the codes themselves are the
+// operand, exactly, and a group's columns have an accumulator of their own, which the epilogue's warps scale and add up in f32 while the
+// next ones are made.  500 rows through 4096 x 4096: 138 us with the taking apart, 501 on the warps' own instructions.
+//
 // What the tiles leave of the last wave is filled by dividing its tiles along the columns: a CTA then leaves its f32 sums in memory, and
 // the last of a tile's CTAs adds them up in their order.  64 rows of bf16 through 4096 x 4096: 17 us, 34 undivided; through 4096 x
 // 11008: 29, 78 undivided; 500 rows of f16 through 11008 x 4096: 62, 67 undivided (whole tiles alone, of 176 rows), where weights
@@ -52,7 +57,7 @@ struct Q4TcParams {
     long long n, rows, k;
     int chunks, groups, group_log2, row_tiles;
     DType scale_dtype;
-    int tile_rows;                       // of x
+    int tile_rows, out_rows;             // of x, and of y that they make
     int tiles_m, tiles_n, stages;
     int whole, shares, share_chunks;     // tiles of one unit each; units of each of the others, and their steps (an even number)
     float* part;                         // sums of those units: [unit][row of x][128]
@@ -107,7 +112,12 @@ template <typename T, bool LOW> __device__ __forceinline__ typename TwoOf<T>::ty
         return __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), __bfloat162bfloat162(__ushort_as_bfloat16(0x4308)));
     }
 }
-template <typename T, bool SAME, bool LOW> __device__ __forceinline__ unsigned two_values(unsigned nib, typename TwoOf<T>::type s2, float s) {
+template <typename T, bool SAME, bool LOW, bool EXACT> __device__ __forceinline__ unsigned two_values(unsigned nib, typename TwoOf<T>::type s2, float s) {
+    if constexpr (EXACT) {
+        const unsigned v = ((LOW ? nib >> 4 : nib) & 0x000f000fu) | 0x3e003e00u;             // (128 + code) / 1024
+        const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), __bfloat162bfloat162(__ushort_as_bfloat16(0x3e08)));
+        return *reinterpret_cast<const unsigned*>(&d);
+    }
     const auto d = less_eight<T, LOW>(nib);
     if constexpr (SAME) {
         const auto v = __hmul2(d, s2);
@@ -141,7 +151,7 @@ __device__ __forceinline__ void store16(unsigned at, uint4 v) {
 
 // A unit as the operand.  `at`: the lane's place for the first of the two halves of a row that it writes; the other is 64
 // bytes away.  `valid`, where the row ends in the unit (ENDS): columns from the lane's first on in the first half.
-template <typename T, bool SAME, bool G32, bool ENDS>
+template <typename T, bool SAME, bool G32, bool EXACT, bool ENDS>
 __device__ __forceinline__ void decode_unit(const Q4Unit<G32>& u, DType scale_dtype, bool odd, unsigned at, int valid) {
     typedef typename TwoOf<T>::type T2;
     const unsigned words[4] = {odd ? u.w.z : u.w.x, odd ? u.w.w : u.w.y, odd ? u.w.x : u.w.z, odd ? u.w.y : u.w.w};
@@ -168,10 +178,10 @@ __device__ __forceinline__ void decode_unit(const Q4Unit<G32>& u, DType scale_dt
             fl = __uint_as_float(raw.x & 0xffff0000u);
         }
         const unsigned a8 = a >> 8, b8 = b >> 8;
-        uint4 top = make_uint4(two_values<T, SAME, false>(a, up, fu), two_values<T, SAME, false>(a8, up, fu), two_values<T, SAME, false>(b, up, fu),
-                               two_values<T, SAME, false>(b8, up, fu));
-        uint4 bottom = make_uint4(two_values<T, SAME, true>(a, low, fl), two_values<T, SAME, true>(a8, low, fl), two_values<T, SAME, true>(b, low, fl),
-                                  two_values<T, SAME, true>(b8, low, fl));
+        uint4 top = make_uint4(two_values<T, SAME, false, EXACT>(a, up, fu), two_values<T, SAME, false, EXACT>(a8, up, fu), two_values<T, SAME, false, EXACT>(b, up, fu),
+                               two_values<T, SAME, false, EXACT>(b8, up, fu));
+        uint4 bottom = make_uint4(two_values<T, SAME, true, EXACT>(a, low, fl), two_values<T, SAME, true, EXACT>(a8, low, fl), two_values<T, SAME, true, EXACT>(b, low, fl),
+                                  two_values<T, SAME, true, EXACT>(b8, low, fl));
         if (ENDS) {
             const int left = valid - 32 * (turn ^ (int)odd);
             top = first_of(top, left);
@@ -182,10 +192,14 @@ __device__ __forceinline__ void decode_unit(const Q4Unit<G32>& u, DType scale_dt
     }
 }
 
-template <typename T, bool SAME, bool G32>
+// EXACT: x in three parts of bf16, whose 32 rows each are the rows of a tile; the codes are the operand, over 1024, and each group's
+// sums are scaled as they are added up, in f32.
+template <typename T, bool SAME, bool G32, bool EXACT>
 __global__ void __launch_bounds__(kThreadsTc, 1) q4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ Q4TcParams p) {
+    typedef typename std::conditional<EXACT, float, T>::type Y;
+    constexpr int kAccs = EXACT ? 4 : 2, kAccCols = 512 / kAccs;
     extern __shared__ unsigned char smem_raw[];
-    __shared__ alignas(8) unsigned long long bars[3 * kMaxStages + 4 + 2 * kPairs];
+    __shared__ alignas(8) unsigned long long bars[3 * kMaxStages + 8 + 2 * kPairs];
     __shared__ unsigned tmem_slot, last;
     const unsigned stages_at = (smem_u32(smem_raw) + 1023) & ~1023u;          // the swizzle wants 1024-byte alignment
     const unsigned stage_bytes = kWBytes + (unsigned)p.tile_rows * kBK * 2;
@@ -195,9 +209,9 @@ __global__ void __launch_bounds__(kThreadsTc, 1) q4_tc_kernel(const __grid_const
     auto w_full = [&](int s) { return bar0 + 8u * (kMaxStages + s); };
     auto empty = [&](int s) { return bar0 + 8u * (2 * kMaxStages + s); };
     auto acc_full = [&](int a) { return bar0 + 8u * (3 * kMaxStages + a); };
-    auto acc_empty = [&](int a) { return bar0 + 8u * (3 * kMaxStages + 2 + a); };
-    auto pair_full = [&](int b) { return bar0 + 8u * (3 * kMaxStages + 4 + b); };
-    auto pair_empty = [&](int b) { return bar0 + 8u * (3 * kMaxStages + 4 + kPairs + b); };
+    auto acc_empty = [&](int a) { return bar0 + 8u * (3 * kMaxStages + 4 + a); };
+    auto pair_full = [&](int b) { return bar0 + 8u * (3 * kMaxStages + 8 + b); };
+    auto pair_empty = [&](int b) { return bar0 + 8u * (3 * kMaxStages + 8 + kPairs + b); };
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int s = 0; s < kMaxStages; ++s) {
@@ -205,7 +219,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) q4_tc_kernel(const __grid_const
             mbar_init(w_full(s), 8);
             mbar_init(empty(s), 1);
         }
-        for (int a = 0; a < 2; ++a) {
+        for (int a = 0; a < kAccs; ++a) {
             mbar_init(acc_full(a), 1);
             mbar_init(acc_empty(a), 4);
         }
@@ -253,11 +267,13 @@ __global__ void __launch_bounds__(kThreadsTc, 1) q4_tc_kernel(const __grid_const
             bool ok = true;
             for (int n = blockIdx.x; n < units && ok; n += gridDim.x) {
                 const Unit u(p, n);
-                if (!mbar_wait(acc_empty(acc), acc_phase)) {
-                    atomicExch(p.error, 82u);
-                    break;
+                if constexpr (!EXACT) {
+                    if (!mbar_wait(acc_empty(acc), acc_phase)) {
+                        atomicExch(p.error, 82u);
+                        break;
+                    }
+                    tc_fence_after();
                 }
-                tc_fence_after();
                 for (int kb = u.begin; kb < u.end; ++kb) {
                     if (!mbar_wait(x_full(stage), phase) || !mbar_wait(w_full(stage), phase)) {
                         atomicExch(p.error, 83u);
@@ -266,49 +282,117 @@ __global__ void __launch_bounds__(kThreadsTc, 1) q4_tc_kernel(const __grid_const
                     }
                     tc_fence_after();
                     const unsigned long long w = first + (unsigned)stage * (stage_bytes >> 4), x = w + (kWBytes >> 4);
+                    if constexpr (EXACT) {
+                        const int inside = (1 << p.group_log2) - 1;
+                        for (int half = 0; half < 2 && ok; ++half) {
+                            const int col = kb * kBK + half * 32;
+                            const bool fresh = (col & inside) == 0;
+                            if (fresh && !mbar_wait(acc_empty(acc), acc_phase)) {
+                                atomicExch(p.error, 82u);
+                                ok = false;
+                                break;
+                            }
+                            tc_fence_after();
+                            umma_f16(tmem + (unsigned)acc * kAccCols, w + 4 * half, x + 4 * half, idesc, !fresh);
+                            umma_f16(tmem + (unsigned)acc * kAccCols, w + 4 * half + 2, x + 4 * half + 2, idesc, 1u);
+                            if (((col + 32) & inside) == 0 || (half && kb + 1 == u.end)) {
+                                umma_commit(acc_full(acc));
+                                if (++acc == kAccs) acc = 0, acc_phase ^= 1;
+                            }
+                        }
+                        if (!ok) break;
+                    } else {
 #pragma unroll
-                    for (int i = 0; i < kBK / 16; ++i) umma_f16(tmem + (unsigned)acc * 256, w + 2 * i, x + 2 * i, idesc, kb != u.begin || i != 0);
+                        for (int i = 0; i < kBK / 16; ++i) umma_f16(tmem + (unsigned)acc * kAccCols, w + 2 * i, x + 2 * i, idesc, kb != u.begin || i != 0);
+                    }
                     umma_commit(empty(stage));
                     if (++stage == p.stages) stage = 0, phase ^= 1;
                 }
-                if (ok) umma_commit(acc_full(acc));
-                if (++acc == 2) acc = 0, acc_phase ^= 1;
+                if constexpr (!EXACT) {
+                    if (ok) umma_commit(acc_full(acc));
+                    if (++acc == kAccs) acc = 0, acc_phase ^= 1;
+                }
             }
         }
     } else if (warp < 6) {
         const int quarter = warp & 3;                 // of the accumulator's lanes
         int acc = 0;
         unsigned acc_phase = 0;
-        for (int i = blockIdx.x; i < units; i += gridDim.x) {
+        bool ok = true;
+        for (int i = blockIdx.x; i < units && ok; i += gridDim.x) {
             const Unit u(p, i);
-            if (!all_of_warp(mbar_wait(acc_full(acc), acc_phase))) {
-                if (lane == 0) atomicExch(p.error, 84u);
-                break;
-            }
-            tc_fence_after();
-            const long long m0 = (long long)(u.tile % p.tiles_m) * p.tile_rows, n = (long long)(u.tile / p.tiles_m) * 128 + quarter * 32 + lane;
-            const int live = (int)min((long long)p.tile_rows, p.rows - m0);
-            T* to = (T*)p.y + m0 * p.n + n;
-            float* mine = u.share < 0 ? nullptr : p.part + (long long)(i - p.whole) * p.tile_rows * 128 + quarter * 32 + lane;
-            for (int c = 0; c < live; c += 32) {
-                unsigned v[32];
-                tmem_ld_32x32(tmem + ((unsigned)(quarter * 32) << 16) + (unsigned)(acc * 256 + c), v);
-                tmem_ld_wait();
+            const long long m0 = (long long)(u.tile % p.tiles_m) * p.out_rows, n = (long long)(u.tile / p.tiles_m) * 128 + quarter * 32 + lane;
+            const int live = (int)min((long long)p.out_rows, p.rows - m0);
+            Y* to = (Y*)p.y + m0 * p.n + n;
+            float* mine = u.share < 0 ? nullptr : p.part + (long long)(i - p.whole) * p.out_rows * 128 + quarter * 32 + lane;
+            // 32 rows of y from c on, of which this lane has column n
+            auto put = [&](int c, auto value) {
                 if (mine) {
 #pragma unroll
                     for (int j = 0; j < 32; ++j)
-                        if (c + j < live) mine[(c + j) * 128] = __uint_as_float(v[j]);
+                        if (c + j < live) mine[(c + j) * 128] = value(j);
                 } else if (n < p.n) {
 #pragma unroll
                     for (int j = 0; j < 32; ++j)
-                        if (c + j < live) to[(c + j) * p.n] = decode::from_f<T>(__uint_as_float(v[j]));
+                        if (c + j < live) to[(c + j) * p.n] = decode::from_f<Y>(value(j));
                 }
                 __syncwarp();
+            };
+            const unsigned from = tmem + ((unsigned)(quarter * 32) << 16);
+            unsigned v[32];
+            if constexpr (EXACT) {
+                float sum[32];
+#pragma unroll
+                for (int j = 0; j < 32; ++j) sum[j] = 0.f;
+                const int first = u.begin * kBK >> p.group_log2, end = ((u.end * kBK - 1) >> p.group_log2) + 1;
+                const long long row = min(n, (long long)p.row_tiles * 16 - 1), at = (row >> 4) * p.groups * 16 + (row & 7) * 2 + (row >> 3 & 1);
+                auto scale = [&](int q) -> float {        // a group behind the last column is all zeros
+                    if (q >= p.groups) return 0.f;
+                    const long long o = at + q * 16;
+                    return p.scale_dtype == DType::F32   ? __ldg((const float*)p.scales + o)
+                           : p.scale_dtype == DType::F16 ? __half2float(__ldg((const __half*)p.scales + o))
+                                                         : __bfloat162float(__ldg((const __nv_bfloat16*)p.scales + o));
+                };
+                float ahead = scale(first);
+                for (int q = first; q < end; ++q) {
+                    const float s = ahead;
+                    if (q + 1 < end) ahead = scale(q + 1);
+                    if (!all_of_warp(mbar_wait(acc_full(acc), acc_phase))) {
+                        if (lane == 0) atomicExch(p.error, 84u);
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+#pragma unroll
+                    for (int part = 0; part < 3; ++part) {
+                        tmem_ld_32x32(from + (unsigned)(acc * kAccCols + part * 32), v);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) sum[j] = fmaf(__uint_as_float(v[j]), s, sum[j]);
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(acc_empty(acc));
+                    if (++acc == kAccs) acc = 0, acc_phase ^= 1;
+                }
+                if (!ok) break;
+                put(0, [&](int j) { return sum[j] * 1024.f; });
+            } else {
+                if (!all_of_warp(mbar_wait(acc_full(acc), acc_phase))) {
+                    if (lane == 0) atomicExch(p.error, 84u);
+                    break;
+                }
+                tc_fence_after();
+                for (int c = 0; c < live; c += 32) {
+                    tmem_ld_32x32(from + (unsigned)(acc * kAccCols + c), v);
+                    tmem_ld_wait();
+                    put(c, [&](int j) { return __uint_as_float(v[j]); });
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(acc_empty(acc));
+                if (++acc == kAccs) acc = 0, acc_phase ^= 1;
             }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(acc_empty(acc));
-            if (++acc == 2) acc = 0, acc_phase ^= 1;
         }
     } else if (warp < 6 + kDecoders) {
         const int d = (warp - 6) & 7, odd = (warp - 6) >> 3;
@@ -347,8 +431,8 @@ __global__ void __launch_bounds__(kThreadsTc, 1) q4_tc_kernel(const __grid_const
                     }
                     const unsigned at = operand + s * stage_bytes;
                     const int valid = (int)p.k - (kb + odd) * kBK - c * 8;
-                    if (valid + c * 8 >= kBK) decode_unit<T, SAME, G32, false>(u, p.scale_dtype, g & 1, at, valid);
-                    else decode_unit<T, SAME, G32, true>(u, p.scale_dtype, g & 1, at, valid);
+                    if (valid + c * 8 >= kBK) decode_unit<T, SAME, G32, EXACT, false>(u, p.scale_dtype, g & 1, at, valid);
+                    else decode_unit<T, SAME, G32, EXACT, true>(u, p.scale_dtype, g & 1, at, valid);
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 }
                 __syncwarp();
@@ -410,21 +494,21 @@ __global__ void __launch_bounds__(kThreadsTc, 1) q4_tc_kernel(const __grid_const
     }
     __syncthreads();
     if (!last) return;
-    const long long m0 = (long long)(u.tile % p.tiles_m) * p.tile_rows, n0 = (long long)(u.tile / p.tiles_m) * 128 + lane * 4;
-    const int live = (int)min((long long)p.tile_rows, p.rows - m0);
-    const float* parts = p.part + (long long)(u.tile - p.whole) * p.shares * p.tile_rows * 128 + lane * 4;
+    const long long m0 = (long long)(u.tile % p.tiles_m) * p.out_rows, n0 = (long long)(u.tile / p.tiles_m) * 128 + lane * 4;
+    const int live = (int)min((long long)p.out_rows, p.rows - m0);
+    const float* parts = p.part + (long long)(u.tile - p.whole) * p.shares * p.out_rows * 128 + lane * 4;
     for (int c = warp; c < live; c += kThreadsTc / 32) {       // a warp has whole rows of x
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
         for (int s = 0; s < p.shares; ++s) {
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(parts + ((long long)s * p.tile_rows + c) * 128));
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(parts + ((long long)s * p.out_rows + c) * 128));
             sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
         }
         const float f[4] = {sum.x, sum.y, sum.z, sum.w};
-        T* row = (T*)p.y + (m0 + c) * p.n + n0;
+        Y* row = (Y*)p.y + (m0 + c) * p.n + n0;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (n0 + e < p.n) row[e] = decode::from_f<T>(f[e]);
+            if (n0 + e < p.n) row[e] = decode::from_f<Y>(f[e]);
     }
     if (threadIdx.x == 0) p.tickets[u.tile - p.whole] = 0;
 }
@@ -434,17 +518,17 @@ __global__ void __launch_bounds__(kThreadsTc, 1) q4_tc_kernel(const __grid_const
 // Tiles of few rows of x cost nearly what tiles of many do, as the time goes into the weights' side: so as few waves as 256 rows
 // allow.  The tiles of the last wave are divided along the columns, where the SMs that they leave would wait, if the adding up
 // costs less.  In us: a step of 64 columns takes 0.44 with 64 rows of x, 0.47 with 128, 0.55 with 256; adding up 2.5, and 0.0105 for
-// each row of x in each share.
-Q4TcPlan q4_tc_plan(Device& dev, const Q4Weight& w, int64_t rows) {
+// each row of x in each share.  Rows of f32: 0.5, with groups of 32 (four accumulators for two steps) 0.8.
+Q4TcPlan q4_tc_plan(Device& dev, const Q4Weight& w, int64_t rows, bool exact) {
     Q4TcPlan best;
-    const int64_t tiles_n = (w.row_tiles + 7) / 8, least = (rows + 255) / 256, sms = dev.sm_count;
+    const int64_t tiles_n = (w.row_tiles + 7) / 8, most_rows = exact ? kExactRows : 256, least = (rows + most_rows - 1) / most_rows, sms = dev.sm_count;
     int64_t before = 0;
-    for (int64_t t = least; t < least + 8; ++t) {
-        const int64_t tile_rows = ((rows + t - 1) / t + 15) / 16 * 16;
+    for (int64_t t = least; t < least + (exact ? 1 : 8); ++t) {
+        const int64_t tile_rows = exact ? kExactRows : ((rows + t - 1) / t + 15) / 16 * 16;
         if (tile_rows == before) continue;
         before = tile_rows;
         const int64_t tiles = tiles_n * ((rows + tile_rows - 1) / tile_rows), whole = tiles / sms * sms, rest = tiles - whole;
-        const double step = 0.40 + 0.0006 * (double)tile_rows, start = 5.0 + (double)(whole / sms * w.chunks) * step;
+        const double step = exact ? (w.group == 32 ? 0.8 : 0.5) : 0.40 + 0.0006 * (double)tile_rows, start = 5.0 + (double)(whole / sms * w.chunks) * step;
         const int most = rest ? (int)std::min<int64_t>(sms / rest, 32) : 1;      // a CTA has one share at most
         for (int s = 1; s <= most; ++s) {
             const int steps = s == 1 ? (int)w.chunks : (((int)w.chunks + s - 1) / s + 1) / 2 * 2, shares = ((int)w.chunks + steps - 1) / steps;
@@ -456,12 +540,13 @@ Q4TcPlan q4_tc_plan(Device& dev, const Q4Weight& w, int64_t rows) {
     return best;
 }
 
-bool q4_tc_run(Device& dev, const Q4Weight& w, const Q4TcPlan& plan, const TensorData& x, int64_t rows, void* y) {
-    const bool bf16 = x.dtype == DType::BF16;
-    const int64_t stride = x.layout.strides[0];
-    if (rows >= (1ll << 31) - 256) return false;              // coordinates of TMA are 32 bits
+bool q4_tc_run(Device& dev, const Q4Weight& w, const Q4TcPlan& plan, const void* x, DType dtype, int64_t stride, int64_t rows, bool exact, void* y) {
+    const bool bf16 = dtype == DType::BF16;
+    const int tile_rows = exact ? 3 * plan.tile_rows : plan.tile_rows;
+    const int64_t x_rows = exact ? (rows + kExactRows - 1) / kExactRows * tile_rows : rows;
+    if (x_rows >= (1ll << 31) - 256) return false;            // coordinates of TMA are 32 bits
     CUtensorMap map;
-    if (!dev.dry && !encode_3d(&map, bf16, x.base_ptr(), w.k, rows, 1, stride, rows * stride, kBK, (unsigned)plan.tile_rows)) return false;
+    if (!dev.dry && !encode_3d(&map, bf16, x, w.k, x_rows, 1, stride, x_rows * stride, kBK, (unsigned)tile_rows)) return false;
     Q4TcParams p{};
     p.codes = (const uint4*)w.codes->ptr;
     p.scales = w.scales->ptr;
@@ -474,12 +559,13 @@ bool q4_tc_run(Device& dev, const Q4Weight& w, const Q4TcPlan& plan, const Tenso
     p.group_log2 = w.group == 32 ? 5 : w.group == 64 ? 6 : 7;
     p.row_tiles = (int)w.row_tiles;
     p.scale_dtype = w.scale_dtype;
-    p.tile_rows = plan.tile_rows;
+    p.tile_rows = tile_rows;
+    p.out_rows = plan.tile_rows;
     p.tiles_m = (int)((rows + plan.tile_rows - 1) / plan.tile_rows);
     p.tiles_n = (int)((w.row_tiles + 7) / 8);
     p.scale_bytes = (int)dtype_size(w.scale_dtype);
     p.tile_bytes = 1024 + (int)(128 / w.group) * 16 * p.scale_bytes;
-    const int stage_bytes = kWBytes + plan.tile_rows * kBK * 2, pairs_bytes = kPairs * 8 * p.tile_bytes;
+    const int stage_bytes = kWBytes + tile_rows * kBK * 2, pairs_bytes = kPairs * 8 * p.tile_bytes;
     p.stages = std::min(kMaxStages, (kRoom - pairs_bytes) / stage_bytes);
     p.error = dev.error_word();
     p.whole = plan.whole;
@@ -488,7 +574,7 @@ bool q4_tc_run(Device& dev, const Q4Weight& w, const Q4TcPlan& plan, const Tenso
     const int64_t divided = (int64_t)p.tiles_m * p.tiles_n - p.whole;     // fewer than SMs
     BufferRef scratch;
     if (p.shares > 1) {
-        scratch = dev.alloc((size_t)(divided * p.shares * p.tile_rows) * 128 * sizeof(float), false);
+        scratch = dev.alloc((size_t)(divided * p.shares * p.out_rows) * 128 * sizeof(float), false);
         p.part = (float*)scratch->ptr;
         p.tickets = (unsigned*)dev.counters();
     }
@@ -500,13 +586,15 @@ bool q4_tc_run(Device& dev, const Q4Weight& w, const Q4TcPlan& plan, const Tenso
             WGF_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRoom + 1024));
             kernel<<<grid, kThreadsTc, smem, dev.stream>>>(map, p);
         };
-        const bool same = w.scale_dtype == x.dtype, g32 = w.group == 32;
-        if (bf16) {
-            if (same) g32 ? go(q4_tc_kernel<__nv_bfloat16, true, true>) : go(q4_tc_kernel<__nv_bfloat16, true, false>);
-            else g32 ? go(q4_tc_kernel<__nv_bfloat16, false, true>) : go(q4_tc_kernel<__nv_bfloat16, false, false>);
+        const bool same = w.scale_dtype == dtype, g32 = w.group == 32;
+        if (exact) {
+            go(q4_tc_kernel<__nv_bfloat16, false, false, true>);
+        } else if (bf16) {
+            if (same) g32 ? go(q4_tc_kernel<__nv_bfloat16, true, true, false>) : go(q4_tc_kernel<__nv_bfloat16, true, false, false>);
+            else g32 ? go(q4_tc_kernel<__nv_bfloat16, false, true, false>) : go(q4_tc_kernel<__nv_bfloat16, false, false, false>);
         } else {
-            if (same) g32 ? go(q4_tc_kernel<__half, true, true>) : go(q4_tc_kernel<__half, true, false>);
-            else g32 ? go(q4_tc_kernel<__half, false, true>) : go(q4_tc_kernel<__half, false, false>);
+            if (same) g32 ? go(q4_tc_kernel<__half, true, true, false>) : go(q4_tc_kernel<__half, true, false, false>);
+            else g32 ? go(q4_tc_kernel<__half, false, true, false>) : go(q4_tc_kernel<__half, false, false, false>);
         }
     }
     dev.end_launch();
