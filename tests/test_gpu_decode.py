@@ -521,17 +521,23 @@ def test_q4_product_of_very_long_rows(kind, wgf, dev):
     close(take(out, kind), *ref.q4_product(x, ref.q4_values(c, s, 128), kind, through=kind))
 
 
-def test_q4_product_on_tensor_cores_replayed(wgf, dev):
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+def test_q4_product_on_tensor_cores_replayed(kind, wgf, dev):
     g = seeded(29, 2)
     rows, n, k = 300, 1100, 1100
-    w, x = draw(g, (n, k), "bf16", 0.02), draw(g, (rows, k), "bf16")
-    t, a = give(wgf, dev, w, "bf16").quantize_q4(64), give(wgf, dev, x, "bf16")
-    want = take(a.mat_mul_q4(t), "bf16")
+    w, x = draw(g, (n, k), "bf16", 0.02), draw(g, (rows, k), kind)
+    t, a = give(wgf, dev, w, kind).quantize_q4(64), give(wgf, dev, x, kind)
+    want = take(a.mat_mul_q4(t), kind)
     with dev.record() as s:
         out = a.mat_mul_q4(t).materialize()
     for _ in range(3):
         s.launch()
-    np.testing.assert_array_equal(take(out, "bf16"), want)
+    np.testing.assert_array_equal(take(out, kind), want)
+    other = draw(g, (rows, k), kind)
+    a.write(ref.store(other, kind))
+    s.launch()
+    want = take(give(wgf, dev, other, kind).mat_mul_q4(t), kind)
+    np.testing.assert_array_equal(take(out, kind), want)
 
 
 @pytest.mark.parametrize("kind", ["f32", "f16"])
