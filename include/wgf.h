@@ -384,10 +384,9 @@ int32_t wgf_q4_weight_release(wgf_q4_weight* w);
 int32_t wgf_q4_weight_info(wgf_q4_weight* w, int64_t* n, int64_t* k, uint32_t* group, uint32_t* scale_dtype);
 /* The values as a [n, k] tensor of `dtype`. */
 int32_t wgf_q4_weight_dequantize(wgf_q4_weight* w, uint32_t dtype, wgf_tensor** out);
-/* x [.., k] times the transposed weights: [.., n] of x's type, lazily.  Up to some dozens of rows
- * are one kernel that reads the codes, with f32 sums of exact products; with more rows of 16 bits the
- * weights' values are rounded to x's type on the way, in the kernel or written out for the matrix
- * product.  Rows of f32 keep exact products. */
+/* x [.., k] times the transposed weights: [.., n] of x's type, lazily, in one kernel (two for many rows of f32, or of
+ * 16 bits that do not begin at 16-byte borders).  f32 sums of exact products for any number of rows and every type: the
+ * weights' values are rounded nowhere on the way, and the result once. */
 int32_t wgf_tensor_matmul_q4(wgf_tensor* x, wgf_q4_weight* w, wgf_tensor** out);
 
 /* ======================================================================================

@@ -760,3 +760,69 @@ def test_kernel_times_of_calls_that_run_at_once(wgf, dev):
     c.append(k, k)
     out = c.attention(k)
     assert out.timing_labels() == ["cache_attention"] and len(out.all_timing_information()) == 1
+
+
+# ---- many rows through 4-bit weights: what is rounded -----------------------------------------------------------------------
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("scale_kind", KINDS)
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("rows,n,k", [(300, 1100, 1100), (257, 1030, 1091), (72, 9000, 2112), (500, 2200, 1985), (1000, 260, 1024), (130, 3000, 64),
+                                      (33, 4100, 40)])
+def test_q4_product_of_many_rows_rounds_sums_alone(kind, scale_kind, group, rows, n, k, wgf, dev):
+    """The weights' values are not rounded to the type of x on the way: the bound is that of f32 sums of exact products."""
+    g = seeded(31, rows + n + k + group)
+    w, x = draw(g, (n, k), scale_kind, 0.02), draw(g, (rows, k), kind)
+    c, s = ref.q4_quantize(w, group, scale_kind)
+    out = take(give(wgf, dev, x, kind).mat_mul_q4(give(wgf, dev, w, scale_kind).quantize_q4(group)), kind)
+    close(out, *ref.q4_product(x, ref.q4_values(c, s, group), kind))
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("rows,n,k", [(2304, 2304, 2051), (2304, 2304, 2048), (4500, 1280, 1030)])
+def test_q4_product_of_very_many_rows_rounds_sums_alone(kind, rows, n, k, wgf, dev):
+    g = seeded(31, rows + k)
+    w, x = draw(g, (n, k), kind, 0.02), draw(g, (rows, k), kind)
+    c, s = ref.q4_quantize(w, 128, kind)
+    dev.set_timing(True)
+    out = give(wgf, dev, x, kind).mat_mul_q4(give(wgf, dev, w, kind).quantize_q4(128))
+    close(take(out, kind), *ref.q4_product(x, ref.q4_values(c, s, 128), kind))
+    assert "q4_tc" in out.timing_labels() and "q4_dequantize" not in out.timing_labels()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows", [9, 17, 33, 100])
+@pytest.mark.parametrize("n,k,group", [(64, 256, 64), (33, 70, 32), (300, 1200, 128)])
+def test_q4_product_in_blocks_rounds_sums_alone(kind, rows, n, k, group, wgf, dev):
+    g = seeded(31, rows + k)
+    w, x = draw(g, (n, k), kind, 0.02), draw(g, (rows, k), kind)
+    c, s = ref.q4_quantize(w, group, kind)
+    dev.set_timing(True)
+    out = give(wgf, dev, x, kind).mat_mul_q4(give(wgf, dev, w, kind).quantize_q4(group))
+    close(take(out, kind), *ref.q4_product(x, ref.q4_values(c, s, group), kind))
+    assert "q4_rows" in out.timing_labels()
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_q4_product_of_very_long_rows_rounds_sums_alone(kind, wgf, dev):
+    g = seeded(31, 4)
+    rows, n, k = 3, 20, 700_040
+    w, x = draw(g, (n, k), kind, 0.02), draw(g, (rows, k), kind)
+    c, s = ref.q4_quantize(w, 128, kind)
+    out = give(wgf, dev, x, kind).mat_mul_q4(give(wgf, dev, w, kind).quantize_q4(128))
+    close(take(out, kind), *ref.q4_product(x, ref.q4_values(c, s, 128), kind))
+
+
+@pytest.mark.parametrize("kind,rows", [("bf16", 300), ("f32", 161), ("f16", 300)])
+def test_q4_product_on_tensor_cores_at_the_ends_of_the_range(kind, rows, wgf, dev):
+    """Rows near the type's largest number, whose sums of a group are finite where the result is."""
+    g = seeded(31, 5)
+    n, k = 1100, 1100
+    top = {"f32": 3e38, "bf16": 3e38, "f16": 6e4}[kind]
+    x = ref.round_to(g.uniform(-1, 1, (rows, k)) * top, kind)
+    c = g.integers(0, 16, (n, k))
+    s = np.full((n, -(-k // 64)), 2.0 ** -20, np.float32)
+    t = dev.q4_weight((c[:, ::2] | c[:, 1::2] << 4).astype(np.uint8), s, k, 64, wgf.F32)
+    dev.set_timing(True)
+    out = give(wgf, dev, x, kind).mat_mul_q4(t)
+    close(take(out, kind), *ref.q4_product(x, ref.q4_values(c - 8, s, 64), kind))
+    assert "q4_tc" in out.timing_labels()

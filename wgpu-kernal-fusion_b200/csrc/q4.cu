@@ -21,10 +21,8 @@
 // measured rate of memory); 16.5 with a CTA for each row tile, whose first loads, staging of x and sums were not
 // overlapped with anything, and 22 where a scale was converted, and so waited for, in the turn that called for it.
 // Seven rows of bf16 through 4096 x 11008: 14.4 us.
-// More rows: in blocks, along the grid's second axis, on the tensor cores (q4_tc.cu), or with the weights written out in the type of
-// x for the matrix product kernels (choose_way has the times).
+// More rows: in blocks, along the grid's second axis, or on the tensor cores (q4_tc.cu; choose_way has the times).
 #include <algorithm>
-#include <cmath>
 
 #include <cooperative_groups.h>
 
@@ -234,9 +232,9 @@ __global__ void q4_split_kernel(const float* __restrict__ x, long long x_stride,
         const long long row = i / pieces, at = (i - row * pieces) * 8;
         uint4 part[3];
         operands<float>(x + row * x_stride, at, k, part);
-        __nv_bfloat16* to = out + (row / kExactRows * 3 * kExactRows + row % kExactRows) * stride + at;
+        __nv_bfloat16* to = out + (row / kSplitRows * 3 * kSplitRows + row % kSplitRows) * stride + at;
 #pragma unroll
-        for (int q = 0; q < 3; ++q) *reinterpret_cast<uint4*>(to + q * kExactRows * stride) = part[q];
+        for (int q = 0; q < 3; ++q) *reinterpret_cast<uint4*>(to + q * kSplitRows * stride) = part[q];
     }
 }
 
@@ -732,21 +730,15 @@ static RowsPlan plan_rows(Device& dev, const Q4Weight& w, int64_t rows, int part
     return best;
 }
 
-// Which way rows take: in blocks through the kernel above, through the tensor cores (q4_tc.cu), or through weights that are
-// written out and the matrix product.  Rows of 16 bits: what each would take is estimated, in us.  Measured, blocks / tensor
-// cores / written out: 11008 x 4096, 64 rows 79 / 35 / 63, 128 rows 116 / 38 / 63, 500 rows 373 / 63 / 80, 2048 rows 1450 / 163 / 145;
-// 4096 x 4096, 20 rows 17 / 18 / 440 (the matrix product of fewer than 64 rows is strided), 64 rows 38 / 20 / 42, 500 rows 179 / 40 / 44;
-// 600 x 4000, 64 rows 12 / 16 / 37, 256 rows 27 / 20 / 38; 1024 x 1024, 64 rows 11 / 13 / 23, 500 rows 27 / 16 / 26.
-// Rows of f32, blocks / tensor cores (as three parts of bf16 each, with the taking apart) / written out for the FFMA product:
-// 4096 x 4096, 500 rows 501 / 138 / 615; 11008 x 4096, 500 rows 1308 / 328 / 1562.
-enum class Q4Way { BLOCKS, TENSOR, WRITTEN };
-static Q4Way choose_way(Device& dev, const RowsPlan& plan, const Q4TcPlan& tc, const Q4Weight& w, int64_t rows, int parts) {
+// Which way rows take: in blocks through the kernel above, or through the tensor cores (q4_tc.cu).  Codes and scales enter both exactly, so that they differ
+// in the order of f32 sums alone.  What each would take is estimated, in us.  Measured, blocks / tensor cores, f16 rows: 11008 x 4096, 32 rows 26 / 38,
+// 48 rows 53 / 38, 500 rows 369 / 62; 4096 x 4096, 32 rows 14 / 16, 48 rows 18 / 17, 500 rows 149 / 32; 600 x 4000 in groups of 32, 100 rows 11 / 17, 500 rows
+// 38 / 25; 1024 x 1024, 200 rows 10 / 11, 500 rows 24 / 13.  f32 rows, with the taking apart: 11008 x 4096, 6 rows 24 / 39, 12 rows 62 / 39;
+// 4096 x 4096, 12 rows 18 / 18, 24 rows 52 / 18; 1024 x 1024, 48 rows 9 / 12, 100 rows 18 / 12.
+enum class Q4Way { BLOCKS, TENSOR };
+static Q4Way choose_way(const RowsPlan& plan, const Q4TcPlan& tc, int parts) {
     const double blocks = plan.shares ? 3.0 + 0.021 * plan.cost : 1e30;
-    if (parts > 1) return blocks <= tc.us + 4.0 ? Q4Way::BLOCKS : Q4Way::TENSOR;      // 4: taking x apart
-    // the matrix product: tiles of 256 x 256 for a pair of SMs, of which half a wave can be cut smaller
-    const double tiles = (double)((rows + 255) / 256) * (double)((w.n + 255) / 256), waves = std::max(1.0, std::ceil(2.0 * tiles / (dev.sm_count / 2)) / 2);
-    const double written = rows < 64 ? 1e30 : 3.0 + 0.55e-6 * (double)w.n * (double)w.k + 8.0 + 0.43 * waves * (double)w.chunks;
-    return blocks <= std::min(tc.us, written) ? Q4Way::BLOCKS : tc.us <= written ? Q4Way::TENSOR : Q4Way::WRITTEN;
+    return blocks <= tc.us + (parts > 1 ? 2.0 : 0.0) ? Q4Way::BLOCKS : Q4Way::TENSOR;      // 2: taking x apart
 }
 
 TensorData run_matmul_q4(Device& dev, const TensorData& x_in, const Q4Weight& w) {
@@ -770,45 +762,35 @@ TensorData run_matmul_q4(Device& dev, const TensorData& x_in, const Q4Weight& w)
     const int parts = x.dtype == DType::F32 ? 3 : 1;
     const RowsPlan plan = plan_rows(dev, w, rows, parts);
     // (rows that one block holds are read off the codes once: nothing is faster)
-    const Q4TcPlan tc = rows > 8 || !plan.shares ? q4_tc_plan(dev, w, rows, parts > 1) : Q4TcPlan();
-    const Q4Way way = choose_way(dev, plan, tc, w, rows, parts);
+    const Q4TcPlan tc = rows > 8 || !plan.shares ? q4_tc_plan(dev, w, rows, parts) : Q4TcPlan();
     dev.note_recorded_buffer(w.codes);
     dev.note_recorded_buffer(w.scales);
-    if (way == Q4Way::TENSOR && parts > 1) {
+    if (choose_way(plan, tc, parts) == Q4Way::TENSOR) {
         if (x.layout.strides[1] != 1 && w.k > 1) x = run_compact(dev, x);
-        const int64_t kp = (w.k + 7) / 8 * 8, tiles = (rows + kExactRows - 1) / kExactRows;
-        BufferRef split = dev.alloc((size_t)(tiles * 3 * kExactRows * kp) * 2, false);
-        out.buf = dev.alloc((size_t)(rows * w.n) * sizeof(float), false);
-        dev.begin_launch("q4_split");
-        if (!dev.dry)
-            q4_split_kernel<<<grid_for(dev, rows * kp / 8), 256, 0, dev.stream>>>((const float*)x.base_ptr(), x.layout.strides[0], rows, w.k, (__nv_bfloat16*)split->ptr, kp);
-        dev.end_launch();
-        if (q4_tc_run(dev, w, tc, split->ptr, DType::BF16, kp, rows, true, out.buf->ptr)) return out;
-    }
-    if (way != Q4Way::BLOCKS) {
-        // rows that begin at 16-byte borders, which the tensor-core kernels want
-        const int64_t kp = parts == 1 ? (w.k + 7) / 8 * 8 : w.k;
-        if (parts == 1 && (kp != w.k || x.layout.strides[1] != 1 || x.layout.strides[0] % 8 || x.layout.strides[0] < w.k || (uintptr_t)x.base_ptr() % 16)) {
+        const int64_t kp = (w.k + 7) / 8 * 8;                 // rows that begin at 16-byte borders
+        out.buf = dev.alloc((size_t)(rows * w.n) * dtype_size(x.dtype), false);
+        if (parts > 1) {
+            const int64_t tiles = (rows + kSplitRows - 1) / kSplitRows;
+            BufferRef split = dev.alloc((size_t)(tiles * 3 * kSplitRows * kp) * 2, false);
+            dev.begin_launch("q4_split");
+            if (!dev.dry)
+                q4_split_kernel<<<grid_for(dev, rows * kp / 8), 256, 0, dev.stream>>>((const float*)x.base_ptr(), x.layout.strides[0], rows, w.k, (__nv_bfloat16*)split->ptr, kp);
+            dev.end_launch();
+            q4_tc_run(dev, w, tc, split->ptr, DType::BF16, kp, rows, parts, out.base_ptr());
+            return out;
+        }
+        if (kp != w.k || x.layout.strides[0] % 8 || x.layout.strides[0] < w.k || (uintptr_t)x.base_ptr() % 16) {
             TensorData wide;
             wide.dtype = x.dtype;
             wide.layout = Layout::contiguous({rows, kp});
-            wide.buf = dev.alloc((size_t)(rows * kp) * dtype_size(x.dtype), true);
+            wide.buf = dev.alloc((size_t)(rows * kp) * dtype_size(x.dtype), false);      // (nothing reads a row behind its last column)
             TensorData window = wide;
             window.layout.shape = {rows, w.k};
             run_copy(dev, window, x);
             x = wide;
         }
-        if (way == Q4Way::TENSOR && parts == 1) {
-            out.buf = dev.alloc((size_t)(rows * w.n) * dtype_size(x.dtype), false);
-            if (q4_tc_run(dev, w, tc, x.base_ptr(), x.dtype, x.layout.strides[0], rows, false, out.base_ptr())) return out;
-        }
-        x.layout.shape = {rows, kp};
-        TensorData full = dequantize_rows(dev, w, x.dtype, kp);
-        full.layout.shape = {kp, w.n};
-        full.layout.strides = {1, kp};
-        TensorData y = run_matmul(dev, x, full);
-        y.layout = out.layout;
-        return y;
+        q4_tc_run(dev, w, tc, x.base_ptr(), x.dtype, x.layout.strides[0], rows, parts, out.base_ptr());
+        return out;
     }
     if (x.layout.strides[1] != 1 && w.k > 1) x = run_compact(dev, x);
     out.buf = dev.alloc((size_t)(rows * w.n) * dtype_size(x.dtype), false);
