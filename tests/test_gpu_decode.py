@@ -826,3 +826,45 @@ def test_q4_product_on_tensor_cores_at_the_ends_of_the_range(kind, rows, wgf, de
     out = give(wgf, dev, x, kind).mat_mul_q4(t)
     close(take(out, kind), *ref.q4_product(x, ref.q4_values(c - 8, s, 64), kind))
     assert "q4_tc" in out.timing_labels()
+
+
+# ---- few rows through 4-bit weights: the codes less 8 enter exactly -----------------------------------------------------------
+def from_codes(wgf, dev, c, s, group):
+    """Weights of codes -8 .. 7 [n, k], k even, and f32 scales."""
+    return dev.q4_weight(((c + 8)[:, ::2] | (c + 8)[:, 1::2] << 4).astype(np.uint8), s, c.shape[1], group, wgf.F32)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows,n,k,group", [(1, 40, 256, 64), (3, 40, 256, 32), (9, 40, 256, 128), (300, 1100, 1100, 64)])
+def test_q4_product_of_an_infinity_is_one(kind, rows, n, k, group, wgf, dev):
+    """An infinite x gives an infinity of the sign that its code has, and NaN only where the code is 8, which stands for zero."""
+    g = seeded(32, rows + k)
+    c = g.integers(-8, 8, (n, k))
+    x = draw(g, (rows, k), kind)
+    x[rows - 1, 70], x[0, 3] = np.inf, -np.inf
+    s = np.full((n, -(-k // group)), 0.01, np.float32)
+    out = take(give(wgf, dev, x, kind).mat_mul_q4(from_codes(wgf, dev, c, s, group)), kind)
+    with np.errstate(invalid="ignore"):
+        infinite = np.where(np.isinf(x), x, 0.0)[:, None, :] * c[None].astype(np.float32)        # 0 * inf is NaN, as it has to be
+        infinite = np.where(np.isinf(x)[:, None, :], infinite, 0.0).sum(-1)
+    np.testing.assert_array_equal(np.isnan(out), np.isnan(infinite))
+    np.testing.assert_array_equal(out[np.isinf(infinite)], infinite[np.isinf(infinite)])
+    assert np.isfinite(out[infinite == 0]).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows,n,k,group", [(1, 40, 256, 64), (2, 33, 512, 32), (7, 100, 256, 128), (12, 40, 256, 64), (300, 1100, 1100, 128)])
+def test_q4_product_of_columns_without_weight(kind, rows, n, k, group, wgf, dev):
+    """Large x in columns whose weights are zero cost the others no digits; a weight that is all zero gives zero itself."""
+    g = seeded(32, rows + n)
+    c = g.integers(-8, 8, (n, k))
+    x = draw(g, (rows, k), kind)
+    for col in range(0, k, 9):
+        c[:, col] = 0
+        x[:, col] = 6e4 if col % 2 else -5e4
+    x = ref.round_to(x, kind)
+    c[5] = 0
+    s = np.full((n, -(-k // group)), 0.01, np.float32)
+    out = take(give(wgf, dev, x, kind).mat_mul_q4(from_codes(wgf, dev, c, s, group)), kind)
+    close(out, *ref.q4_product(x, ref.q4_values(c, s, group), kind))
+    assert not out[:, 5].any()

@@ -11,7 +11,7 @@
 // The scales of a tile's 16 rows stand together for each group, those of rows g and g + 8 side by side.
 //
 // Few rows of x: every weight is read once, half a byte each, and used for at most a few multiplications, so memory is the
-// bound, and next to it the instructions that turn words into operands (about 65 of f16 and 85 of bf16 for the 16 x 64 weights of a
+// bound, and next to it the instructions that turn words into operands (about 80 of f16 and 85 of bf16 for the 16 x 64 weights of a
 // unit; 11008 x 4096 weights are 74 units for each scheduler of the GPU).  The instruction's eight columns are the
 // rows of x; codes become f16 or bf16 exactly, and sums are f32 within a group and across groups.  A row of f32 takes
 // three columns: its bf16 parts, which together have its 24 bits.  The product does not go through tensor memory: for
@@ -246,12 +246,10 @@ template <bool WIDE> __device__ __forceinline__ float2 two_scales(unsigned at, b
     return make_float2(half ? h.x : __uint_as_float(v << 16), half ? h.y : __uint_as_float(v & 0xffff0000u));
 }
 
-// A word's codes as the operand of one instruction.
-// bf16: (code - 8) / 1024, exactly.  x may be anywhere in the range of f32, and sums of 128 products must not leave it.
-// f16: the nibbles where they are, as the smallest numbers of the type: code * 2^-24 in rows g, and 16 times that in rows
-// g + 8, whose nibbles stand four bits higher.  No bit has to move for it but by a shift of eight.  The 8 is taken off by
-// starting the sums from -8 times the sum of x, which is the same for all rows (constant_rows is the operand that gives it),
-// and the powers of two at the end of a stretch.
+// A word's codes less 8 as the operand of one instruction, exactly.
+// bf16: (code - 8) / 1024.  x may be anywhere in the range of f32, and sums of 128 products must not leave it.
+// f16: the nibbles of rows g under the exponent of 1024, less 1032; those of rows g + 8 stand four bits higher, so there it is a
+// sixteenth of 1024 + 16 code, less 72, as one fused multiply-add.
 template <bool BF> __device__ __forceinline__ void expand(unsigned w, unsigned (&a)[4]) {
     if constexpr (BF) {
         const __nv_bfloat162 off = __halves2bfloat162(__ushort_as_bfloat16(0xbe08), __ushort_as_bfloat16(0xbe08));    // -136 / 1024
@@ -262,18 +260,17 @@ template <bool BF> __device__ __forceinline__ void expand(unsigned w, unsigned (
             a[i] = *reinterpret_cast<const unsigned*>(&d);
         }
     } else {
-        const unsigned u = w >> 8;
-        a[0] = w & 0x000f000fu;
-        a[1] = w & 0x00f000f0u;
-        a[2] = u & 0x000f000fu;
-        a[3] = u & 0x00f000f0u;
+        const __half2 off = __half2half2(__ushort_as_half(0xe408)), sixteenth = __half2half2(__ushort_as_half(0x2c00)), low = __half2half2(__ushort_as_half(0xd480));
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+            const unsigned u = i ? w >> 8 : w, x = (u & 0x000f000fu) | 0x64006400u, y = (u & 0x00f000f0u) | 0x64006400u;
+            const __half2 d = __hadd2(*reinterpret_cast<const __half2*>(&x), off), e = __hfma2(*reinterpret_cast<const __half2*>(&y), sixteenth, low);
+            a[i] = *reinterpret_cast<const unsigned*>(&d);
+            a[i + 1] = *reinterpret_cast<const unsigned*>(&e);
+        }
     }
 }
-__device__ __forceinline__ void constant_rows(unsigned (&a)[4]) {
-    a[0] = a[1] = a[2] = a[3] = 0x80088008u;     // -8 * 2^-24
-}
-template <bool BF> __device__ __forceinline__ float upper_unit() { return BF ? 1024.f : 0x1p24f; }    // rows g
-template <bool BF> __device__ __forceinline__ float lower_unit() { return BF ? 1024.f : 0x1p20f; }    // rows g + 8
+template <bool BF> __device__ __forceinline__ float operand_unit() { return BF ? 1024.f : 1.f; }
 
 template <bool BF> __device__ __forceinline__ void mma(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1, bool fresh) {
     // fresh: the accumulator starts from zero
@@ -305,8 +302,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) q4_rows_kernel(const __grid_co
     extern __shared__ __align__(16) unsigned char smem[];
     unsigned char* ring = smem + (threadIdx.x >> 5) * (DEPTH * UNIT);   // [unit]{ 512 bytes of words; the lanes' scales }
     uint4* xs = reinterpret_cast<uint4*>(smem + kWarps * DEPTH * UNIT); // [chunk][half][column][4], and 16 bytes of zeros
-    float* start = reinterpret_cast<float*>(xs + p.share_chunks * p.columns * 8 + 1);    // f16: [chunk][half][COLS]
-    float* sums = start + (BF ? 0 : p.share_chunks * 2 * COLS);         // [slot][row][column]
+    float* sums = reinterpret_cast<float*>(xs + p.share_chunks * p.columns * 8 + 1);     // [slot][row][column]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     cg::cluster_group cluster = cg::this_cluster();
     const int shares = (int)cluster.num_blocks(), share = (int)cluster.block_rank();
@@ -389,32 +385,14 @@ __global__ void __launch_bounds__(kWarps * 32, 1) q4_rows_kernel(const __grid_co
         x0[n] = shared_address(have ? xs + n * 32 + lane : xs + nk * 8 * p.columns);
         x_step[n] = have ? p.columns * 128 : 0;
     }
-    if constexpr (!BF) {
-        // -8 * 2^-24 times the sums of x over each group of a chunk
-        unsigned a[4];
-        constant_rows(a);
-        for (int k = warp; k < nk; k += kWarps) {
-            float acc[CT][4];
-#pragma unroll
-            for (int half = 0; half < 2; ++half)
-#pragma unroll
-                for (int n = 0; n < CT; ++n) {
-                    const uint4 x = shared_16(x0[n] + k * x_step[n] + (half ? x_step[n] / 2 : 0));
-                    mma<BF>(acc[n], a, x.x, x.y, half == 0 || G32);
-                    mma<BF>(acc[n], a, x.z, x.w, false);
-                    if (g == 0) *reinterpret_cast<float2*>(start + (k * 2 + half) * COLS + n * 8 + c * 2) = make_float2(acc[n][0], acc[n][1]);
-                }
-        }
-        __syncthreads();
-    }
     const bool half_scales = p.scale_dtype == DType::F16;
     float* put = sums + (tile + warp) * SLOT + g * COLS + c * 2;       // every (tile, warp) that meet have a slot of their own
     auto put_down = [&] {
-        const float up = upper_unit<BF>(), low = lower_unit<BF>();
+        const float unit = operand_unit<BF>();
 #pragma unroll
         for (int n = 0; n < CT; ++n) {
-            *reinterpret_cast<float2*>(put + n * 8) = make_float2(total[n][0] * up, total[n][1] * up);
-            *reinterpret_cast<float2*>(put + 8 * COLS + n * 8) = make_float2(total[n][2] * low, total[n][3] * low);
+            *reinterpret_cast<float2*>(put + n * 8) = make_float2(total[n][0] * unit, total[n][1] * unit);
+            *reinterpret_cast<float2*>(put + 8 * COLS + n * 8) = make_float2(total[n][2] * unit, total[n][3] * unit);
             total[n][0] = total[n][1] = total[n][2] = total[n][3] = 0.f;
         }
         put += SLOT;
@@ -426,7 +404,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) q4_rows_kernel(const __grid_co
         // a tile's units
         const int stretch = min(nk - at, mine - done);
         done += stretch;
-        unsigned xl[CT], from = shared_address(start) + (at * 2 * COLS + c * 2) * 4;
+        unsigned xl[CT];
 #pragma unroll
         for (int n = 0; n < CT; ++n) xl[n] = x0[n] + at * x_step[n];
         at = 0;
@@ -443,24 +421,10 @@ __global__ void __launch_bounds__(kWarps * 32, 1) q4_rows_kernel(const __grid_co
                 uint4 x[CT];
 #pragma unroll
                 for (int n = 0; n < CT; ++n) x[n] = shared_16(xl[n] + (half ? x_step[n] / 2 : 0));
-                if constexpr (!BF) {
-                    // rows g + 8 count in units 16 times as large
-                    if (half == 0 || G32) {
-#pragma unroll
-                        for (int n = 0; n < CT; ++n) {
-                            const float2 v = shared_float2(from + ((G32 ? half : 1) * COLS + n * 8) * 4);
-                            acc[half][n][0] = v.x;
-                            acc[half][n][1] = v.y;
-                            acc[half][n][2] = v.x * 16.f;
-                            acc[half][n][3] = v.y * 16.f;
-                        }
-                    }
-                }
-                const bool fresh = BF || (half == 1 && !G32);
                 unsigned a[4];
                 expand<BF>(half ? words.z : words.x, a);
 #pragma unroll
-                for (int n = 0; n < CT; ++n) mma<BF>(acc[half][n], a, x[n].x, x[n].y, fresh);
+                for (int n = 0; n < CT; ++n) mma<BF>(acc[half][n], a, x[n].x, x[n].y, true);
                 expand<BF>(half ? words.w : words.y, a);
 #pragma unroll
                 for (int n = 0; n < CT; ++n) mma<BF>(acc[half][n], a, x[n].z, x[n].w, false);
@@ -472,7 +436,6 @@ __global__ void __launch_bounds__(kWarps * 32, 1) q4_rows_kernel(const __grid_co
             if (slot >= ring_end) slot -= DEPTH * UNIT;
 #pragma unroll
             for (int n = 0; n < CT; ++n) xl[n] += x_step[n];
-            from += 2 * COLS * 4;
 #pragma unroll
             for (int n = 0; n < CT; ++n)
 #pragma unroll
@@ -525,7 +488,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) q4_rows_kernel(const __grid_co
 
 // Shared memory of a CTA whose warps have `depth` units on their way
 size_t rows_smem(int share_chunks, int columns, int tiles, int ct, int shares, int unit, int depth) {
-    return (size_t)kWarps * depth * unit + (size_t)share_chunks * (columns * 128 + ct * 64) + 16 +
+    return (size_t)kWarps * depth * unit + (size_t)share_chunks * (columns * 128) + 16 +
            (size_t)(tiles + kWarps + (shares > 1 ? tiles : 0)) * 16 * ct * 8 * sizeof(float);
 }
 
