@@ -363,7 +363,9 @@ int32_t wgf_kv_cache_append_qk(wgf_kv_cache* cache, wgf_tensor* q, wgf_tensor* k
  * head h reads kv head h * kv_heads / heads).  The queries stand at the last positions of their sequence
  * (with `counts`, the first counts[b] of them do and the others are padding) and each sees the tokens up
  * to its own.  A query before the sequence's first token, and a padding one, gives zeros.  Made for a
- * few tokens a sequence; scores, sums and products are f32 for every element type. */
+ * few tokens a sequence; for every element type scores and sums are f32, and queries and probabilities
+ * enter the products with 22 bits (a probability with what is above 2^-40 of its row's largest).  Values are
+ * weighted and added up before the sum is divided: those above 3e38 / tokens may come out infinite. */
 int32_t wgf_kv_cache_attention(wgf_kv_cache* cache, wgf_tensor* q, float scale, const int64_t* counts, wgf_tensor** out);
 /* The values that the codes stand for: two tensors [batch, kv_heads, longest length, head_dim], zero
  * behind each sequence's end. */

@@ -101,9 +101,9 @@ def attention(q, k, v, scale, count=None, kind="f32"):
             total = p.sum()
             ref[h, i] = p @ vv[:m] / total
             # probabilities: two scores' errors each way, the exponential, the rescalings of the running maximum
-            # (one a block and two joins), the sums of m / 16 steps; what is below 2^-25 of the largest may be lost
+            # (one a block and two joins), the sums of m / 16 steps; of a small probability 2^-40 of the largest may be lost
             rel = 2 * ds.max() * 1.01 + (m / 16 + m / BLOCK + 40) * 2.0 ** -23
-            bound[h, i] = 2 * rel * (p @ np.abs(vv[:m])) / total + 2.0 ** -24 * np.abs(vv[:m]).sum(0) / total
+            bound[h, i] = 2 * rel * (p @ np.abs(vv[:m])) / total + 2.0 ** -39 * np.abs(vv[:m]).sum(0) / total
     return ref, bound + rounding(ref, kind)
 
 

@@ -868,3 +868,27 @@ def test_q4_product_of_columns_without_weight(kind, rows, n, k, group, wgf, dev)
     out = take(give(wgf, dev, x, kind).mat_mul_q4(from_codes(wgf, dev, c, s, group)), kind)
     close(out, *ref.q4_product(x, ref.q4_values(c, s, group), kind))
     assert not out[:, 5].any()
+
+
+# ---- attention: small probabilities beside a dominant one ---------------------------------------------------------------------
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("gap", [5.0, 11.0, 14.0, 17.5])
+@pytest.mark.parametrize("lengths,spread", [([900], 0.0), ([8001, 2000], 0.0), ([8001], 1.0), ([60000], 0.0)])
+def test_cache_attention_behind_a_dominant_key(kind, gap, lengths, spread, wgf, dev):
+    """The first key takes nearly all of the weight and its value is zero: the result is what the others' small weights bring."""
+    g = seeded(33, int(gap) + lengths[0])
+    b, n, d = len(lengths), max(lengths), 64
+    k = np.zeros((b, 1, n, d), np.float32)
+    k[..., 0] = g.standard_normal((b, 1, n)) * spread
+    k[:, :, 0, 0] = gap
+    v = g.standard_normal((b, 1, n, d)) + 1.0
+    v[:, :, 0] = 0
+    q = np.zeros((b, 2, 1, d), np.float32)
+    q[..., 0] = [[[1.0], [0.75]]]
+    k, v = ref.round_to(k, kind), ref.round_to(v, kind)
+    c = dev.kv_cache(b, 1, d, n, code_of(wgf, kind))
+    c.append(give(wgf, dev, k, kind), give(wgf, dev, v, kind), counts=lengths)
+    out = take(c.attention(give(wgf, dev, q, kind), scale=1.0), kind)
+    for i, m in enumerate(lengths):
+        want, bound = ref.attention(q[i], ref.stands_for(k[i, 0, :m])[None], ref.stands_for(v[i, 0, :m])[None], 1.0)
+        close(out[i], want, bound + ref.rounding(want, kind))

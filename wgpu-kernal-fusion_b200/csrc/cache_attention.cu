@@ -12,8 +12,10 @@
 //     copies the bytes that it will read itself (16 at a time, asynchronously, three half blocks in flight).
 //   * Codes become f16 exactly: the byte is put under the exponent of 1024 and 1152 is taken off.
 //   * The 16 rows of the instruction are 8 query rows twice: the f16 nearest to the value and the f16 nearest to what
-//     that leaves.  Queries (scaled by a power of two of their own) and probabilities so keep 22 bits, for all element
-//     types alike, at no cost: eight rows are as many as grouped heads commonly have.
+//     that leaves.  Both kinds are first brought to the upper end of the type's range, queries by a power of two of their own,
+//     probabilities by 2^15: what the two f16 lose is 2^-22 of a value, or 2^-38 of the row's largest one where that is more.  So many
+//     small probabilities beside a dominant one keep their digits, for all element types alike, at no cost: eight rows are as
+//     many as grouped heads commonly have.
 //   * The lane that holds the scores of a row's tokens is the lane that needs them as the A operand of the second
 //     product, because tokens are numbered so (key_token in kv_cache.cu): nothing is exchanged between the products.
 //   * The work of all sequences, heads and row tiles is laid end to end in units of four blocks (one for each warp of
@@ -40,6 +42,7 @@ constexpr int kGiven = 256;
 constexpr int kRows = 8;        // query rows of a tile
 constexpr int kMaxBatch = 1024; // sequences whose work is shared out evenly
 constexpr int kStages = 3;      // half blocks (keys or values of 64 tokens) in a warp's ring
+constexpr float kProbUp = 32768.f;   // probabilities, at most 1, go to the upper end of f16 before they are split
 
 struct AttParams {
     const uint8_t* codes;
@@ -301,13 +304,13 @@ __global__ void __launch_bounds__(kWarps * 32) cache_attention_kernel(const __gr
             for (int n = 0; n < 8; ++n) {
                 const float p0 = exp2f(s[n][0] - from), p1 = exp2f(s[n][1] - from);
                 sum += p0 + p1;
-                split_f16(p0, p1, ph[n], pl[n]);
+                split_f16(p0 * kProbUp, p1 * kProbUp, ph[n], pl[n]);
             }
             l = l * keep + sum;                                // this lane's tokens; the four lanes are added at the end
 
             copies_wait<kStages - 2>();
             const unsigned char* vb = ring + ((2 * it + 1) % kStages) * (kBlock * DP);
-            const float vs = room > 0 ? sc.y : 0.f;            // a row that sees nothing of the block takes nothing of its scale
+            const float vs = room > 0 ? sc.y * (1.f / kProbUp) : 0.f;            // a row that sees nothing of the block takes nothing of its scale
 #pragma unroll
             for (int i = 0; i < ND; ++i) {
                 const uint4 w = *reinterpret_cast<const uint4*>(vb + i * 512);
