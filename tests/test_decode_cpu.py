@@ -283,3 +283,18 @@ def test_cpp_mirror_without_gpu(cpp_binary):
 @pytest.mark.gpu
 def test_cpp_mirror_on_gpu(cpp_binary):
     run_cpp(cpp_binary)
+
+
+@pytest.mark.parametrize("rows", [0, 5])
+def test_fused_append_of_padding_alone_reads_no_tables(wgf, drydev, rows):
+    """No sequence has or takes a token: the tables may be empty, so no kernel may look at them."""
+    c = drydev.kv_cache(2, 2, 64, 100, wgf.F16)
+    q, k = blank(wgf, drydev, (2, 6, 3, 64)), blank(wgf, drydev, (2, 2, 3, 64))
+    w, t = blank(wgf, drydev, (64,)), blank(wgf, drydev, (rows, 32))
+    before = drydev.launch_count
+    out = c.append_qk(q, k, k, w, w, t, t, counts=[0, 0])
+    assert out.shape == (2, 6, 3, 64) and c.lengths == [0, 0] and drydev.launch_count == before
+    if rows == 0:
+        refused(wgf, "SHAPE", c.append_qk, q, k, k, w, w, t, t, counts=[0, 1])
+        refused(wgf, "SHAPE", c.append_qk, q, k, k, w, w, t, t)
+    assert c.lengths == [0, 0]

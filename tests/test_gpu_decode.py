@@ -892,3 +892,15 @@ def test_cache_attention_behind_a_dominant_key(kind, gap, lengths, spread, wgf, 
     for i, m in enumerate(lengths):
         want, bound = ref.attention(q[i], ref.stands_for(k[i, 0, :m])[None], ref.stands_for(v[i, 0, :m])[None], 1.0)
         close(out[i], want, bound + ref.rounding(want, kind))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows", [0, 7])
+def test_fused_append_of_padding_alone_gives_zeros(kind, rows, wgf, dev):
+    c = dev.kv_cache(2, 1, 64, 20, code_of(wgf, kind))
+    bad = give(wgf, dev, np.full((2, 1, 3, 64), np.nan, np.float32), kind)
+    q = give(wgf, dev, np.full((2, 4, 3, 64), np.nan, np.float32), kind)
+    w, t = give(wgf, dev, np.ones(64, np.float32), kind), give(wgf, dev, np.ones((rows, 32), np.float32), kind)
+    for _ in range(2):
+        assert not take(c.append_qk(q, bad, bad, w, w, t, t, counts=[0, 0]), kind).any()
+    assert c.lengths == [0, 0] and c.read()[0].shape == (2, 1, 0, 64)

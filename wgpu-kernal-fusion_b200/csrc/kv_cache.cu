@@ -569,7 +569,8 @@ TensorData append(KvCache& c, const TensorData& k_in, const TensorData& v_in, co
         out.layout = Layout::contiguous(qs);
     }
     dev.make_current();
-    if (q_in) out.buf = dev.alloc((size_t)std::max<int64_t>(out.layout.numel(), 1) * dtype_size(c.dtype), false);
+    if (q_in) out.buf = dev.alloc((size_t)std::max<int64_t>(out.layout.numel(), 1) * dtype_size(c.dtype), most == 0);
+    if (most == 0) return out;     // no sequence has or takes a token: q is padding, and cos / sin may be empty
     if (t == 0) return out;
     auto last_dense = [&](const TensorData& x) {
         const int l = x.layout.rank() - 1;
