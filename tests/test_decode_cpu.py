@@ -298,3 +298,26 @@ def test_fused_append_of_padding_alone_reads_no_tables(wgf, drydev, rows):
         refused(wgf, "SHAPE", c.append_qk, q, k, k, w, w, t, t, counts=[0, 1])
         refused(wgf, "SHAPE", c.append_qk, q, k, k, w, w, t, t)
     assert c.lengths == [0, 0]
+
+
+def test_a_recording_that_is_broken_off_counts_what_it_recorded(wgf, drydev):
+    """A call inside fails and the block is left: what was recorded before it has run once, and the refused call has left nothing."""
+    c = drydev.kv_cache(1, 1, 64, 8, wgf.F16)
+    k = blank(wgf, drydev, (1, 1, 1, 64))
+    for refusal in (dict(counts=[1]), None):
+        before = c.lengths[0]
+        with pytest.raises(wgf.WgfError):
+            with drydev.record():
+                c.append(k, k)
+                if refusal:
+                    c.append(k, k, **refusal)
+                c.truncate([0])
+        assert c.lengths == [before + 1]
+    with pytest.raises(wgf.WgfError):
+        with drydev.record():
+            c.append(blank(wgf, drydev, (1, 1, 7, 64)), k)
+    assert c.lengths == [2]
+    with drydev.record() as s:
+        c.append(k, k)
+    s.launch()
+    assert c.lengths == [4]

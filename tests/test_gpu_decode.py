@@ -904,3 +904,23 @@ def test_fused_append_of_padding_alone_gives_zeros(kind, rows, wgf, dev):
     for _ in range(2):
         assert not take(c.append_qk(q, bad, bad, w, w, t, t, counts=[0, 0]), kind).any()
     assert c.lengths == [0, 0] and c.read()[0].shape == (2, 1, 0, 64)
+
+
+def test_a_recording_that_is_broken_off_keeps_host_and_device_together(wgf, dev):
+    g = seeded(34, 1)
+    k, v, q = draw(g, (1, 2, 9, 64), "f16", 2.0), draw(g, (1, 2, 9, 64), "f16"), draw(g, (1, 2, 1, 64), "f16")
+    t = lambda x, a, b: dev.tensor(ref.store(x[:, :, a:b], "f16"))
+    c, plain = (dev.kv_cache(1, 2, 64, 12, wgf.F16) for _ in range(2))
+    parts = [(t(k, a, b), t(v, a, b)) for a, b in ((0, 3), (3, 4), (4, 9))]
+    tq = dev.tensor(ref.store(q, "f16"))
+    c.append(*parts[0])
+    with pytest.raises(wgf.WgfError):
+        with dev.record():
+            c.append(*parts[1])
+            c.attention(tq, counts=[1])          # fixed numbers: refused
+    assert c.lengths == [4]
+    c.append(*parts[2])
+    plain.append(t(k, 0, 9), t(v, 0, 9))
+    assert c.lengths == plain.lengths == [9]
+    for a, b in zip(contents(c, tq, "f16"), contents(plain, tq, "f16")):
+        np.testing.assert_array_equal(a, b)
