@@ -447,7 +447,8 @@ int32_t wgf_schedule_end(wgf_device* dev, wgf_schedule** out);
 int32_t wgf_schedule_launch(wgf_schedule* s);
 /* Kernels (and copies) one launch runs. */
 int32_t wgf_schedule_kernel_count(wgf_schedule* s, uint64_t* out);
-/* Waits for replays in flight, then frees the graph and returns its memory to the pool. */
+/* Waits for replays in flight, then frees the graph and returns its memory to the pool.  Allowed while another
+ * schedule is being recorded. */
 int32_t wgf_schedule_destroy(wgf_schedule* s);
 
 /* ======================================================================================

@@ -924,3 +924,20 @@ def test_a_recording_that_is_broken_off_keeps_host_and_device_together(wgf, dev)
     assert c.lengths == plain.lengths == [9]
     for a, b in zip(contents(c, tq, "f16"), contents(plain, tq, "f16")):
         np.testing.assert_array_equal(a, b)
+
+
+def test_a_schedule_may_go_while_another_is_recorded(wgf, dev):
+    """The name of the last schedule is bound anew inside the next one's block, so that the old one is destroyed while the new one is recorded."""
+    g = seeded(34, 2)
+    k, q = draw(g, (1, 1, 200, 64), "f16"), draw(g, (1, 2, 1, 64), "f16")
+    c = dev.kv_cache(1, 1, 64, 200, wgf.F16)
+    tk, tq = dev.tensor(ref.store(k, "f16")), dev.tensor(ref.store(q, "f16"))
+    c.append(tk, tk)
+    want = c.attention(tq).as_slice()
+    for _ in range(3):
+        with dev.record() as s:
+            out = c.attention(tq) * 2.0
+            out.materialize()
+        for _ in range(2):
+            s.launch()
+        np.testing.assert_array_equal(ref.load(out.as_slice(), "f16"), ref.load(want, "f16") * 2)

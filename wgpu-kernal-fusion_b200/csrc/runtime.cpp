@@ -730,8 +730,9 @@ void Device::replay(const Recorded& r) {
 void Device::destroy_recorded(Recorded& r) {
     if (!dry) {
         cudaSetDevice(ordinal);
-        // a replay may still be running: its memory must not reach the pool before it ends
-        if (r.exec) cudaStreamSynchronize(stream);
+        // a replay may still be running: its memory must not reach the pool before it ends.  (While another schedule is being
+        // recorded none is, and a wait would end that recording.)
+        if (r.exec && !recording()) cudaStreamSynchronize(stream);
         if (r.exec) cudaGraphExecDestroy(r.exec);
         if (r.graph) cudaGraphDestroy(r.graph);
     }
