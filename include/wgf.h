@@ -325,9 +325,9 @@ int32_t wgf_tensor_graph_size(wgf_tensor* t, uint64_t* nodes);
  *
  * A cache holds `batch` sequences of up to `capacity` tokens.  Each block of 64 tokens of one
  * kv head has one scale for its keys and one for its values: scale = max|x| / 127, code =
- * 127 x / max|x| rounded to the nearest, ties to even (max|x| is taken as 2^-100 at least; a
- * block with a value that is not finite gets a NaN scale, which reaches every query that sees
- * the block).  The block that is still open is coded anew, from its tokens' own values, with
+ * 127 x / max|x| rounded to the nearest, ties to even (max|x| is taken as 2^-100 at least, and 127 times
+ * the scale stays finite; a block with a value that is not finite gets a NaN scale, which reaches every
+ * query that sees the block).  The block that is still open is coded anew, from its tokens' own values, with
  * every append: what the cache holds depends on the tokens and not on the calls that brought
  * them.  Cache calls run at once, in the order in which they are made (a lazy operand is
  * materialised first); they take tensors of the cache's element type, of any strides.

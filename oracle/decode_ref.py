@@ -69,7 +69,7 @@ def codes(x):
             continue
         top = max(np.abs(part).max(), 2.0 ** -100)
         out[b * BLOCK: (b + 1) * BLOCK] = np.rint(127.0 * part / top)
-        scales[b] = np.float32(top) / np.float32(127)
+        scales[b] = min(np.float32(top) / np.float32(127), np.float32(float.fromhex("0x1.020406p+121")))     # 127 times it is finite
     return out, scales
 
 

@@ -941,3 +941,24 @@ def test_a_schedule_may_go_while_another_is_recorded(wgf, dev):
         for _ in range(2):
             s.launch()
         np.testing.assert_array_equal(ref.load(out.as_slice(), "f16"), ref.load(want, "f16") * 2)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("sign", [1, -1])
+def test_cache_of_the_largest_numbers_is_finite(kind, sign, wgf, dev):
+    """A token of the type's largest (or lowest) number does not come back as an infinity."""
+    top = {"f32": float(np.finfo(np.float32).max), "f16": 65504.0, "bf16": float.fromhex("0x1.fep+127")}[kind]
+    g = seeded(35, 1)
+    x = draw(g, (1, 1, 70, 64), kind)
+    x[0, 0, 3], x[0, 0, 66, 5] = sign * top, top
+    c = dev.kv_cache(1, 1, 64, 70, code_of(wgf, kind))
+    c.append(give(wgf, dev, x, kind), give(wgf, dev, -x, kind))
+    for got, want in zip(c.read(), (x, -x)):
+        got = take(got, kind)
+        assert np.isfinite(got).all()
+        np.testing.assert_array_equal(got, ref.round_to(kept(want, [70]), kind))
+    # the only key that a query sees: its value
+    one = dev.kv_cache(1, 1, 64, 70, code_of(wgf, kind))
+    one.append(give(wgf, dev, x[:, :, 3:4] * 0, kind), give(wgf, dev, x[:, :, 3:4], kind))
+    out = take(one.attention(give(wgf, dev, x[:, :, :1], kind)), kind)
+    np.testing.assert_array_equal(out[0, 0, 0], ref.round_to(ref.stands_for(x[0, 0, 3:4]), kind)[0])

@@ -296,7 +296,8 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_consta
                         out[(d >> 3) * 32 + ((d & 7) + e) * 4 + c4] = finite ? make_uint4(w[e][0], w[e][1], w[e][2], w[e][3]) : none;
                 }
             }
-            if (threadIdx.x == 0) *c.scale(b, h, blk, kv) = finite ? amax / 127.f : __uint_as_float(0x7fc00000u);
+            // 127 times the quotient of the largest f32 would round to infinity: that one scale is the number below
+            if (threadIdx.x == 0) *c.scale(b, h, blk, kv) = finite ? fminf(amax / 127.f, 0x1.020406p+121f) : __uint_as_float(0x7fc00000u);
             if (blk == first_blk && p.t > 0) {
                 for (int x = max(open - 1, first_blk + 1); x <= open; ++x)
                     if (!((x ^ first_blk) & 1) && x * kBlock < end) {
