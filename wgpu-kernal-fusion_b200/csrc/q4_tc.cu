@@ -4,7 +4,7 @@
 //
 // The codes less 8 are the A operand, exactly, and the rows of x the B operand: every product is exact, a group's columns have an accumulator
 // of their own, and the scale enters in f32 when the group's sum is added to the others.  Rounded are f32 sums, and y once.  (Weights that are
-// rounded to 16 bits on the way would need neither the accumulators nor the adding up; they lose a quarter of the result's digits beyond its own rounding.)
+// rounded to 16 bits on the way would need neither the accumulators nor the adding up; for f16 the result's error is then a quarter larger.)
 //
 // A tile is 128 rows of the weights by up to 256 rows of x, whose number is chosen so that the tiles fill the SMs (q4_tc_plan).  Warp roles of a CTA,
 // one CTA a SM:
@@ -24,12 +24,12 @@
 // What the tiles leave of the last wave is filled by dividing its tiles along the columns: a CTA then leaves its f32 sums in memory, and
 // the last of a tile's CTAs adds them up in their order, eight rows side by side (a row after the other took 27 us for six shares of 250 rows, eight 2).
 //
-// 500 rows of f16 through 11008 x 4096: 62 us with groups of 128, 74 with groups of 64, 118 with groups of 32; 64 rows of bf16 through 4096 x 4096: 17;
+// 500 rows of f16 through 11008 x 4096: 62 us with groups of 128, 68 with groups of 64, 109 with groups of 32; 64 rows of bf16 through 4096 x 4096: 17;
 // 500 rows of f32 through 4096 x 4096: 145 with the taking apart.  The products alone would take 27 for the first at the measured rate of the tensor cores.
-// With groups of 128 x bounds it: 32 KB a step for every SM are 9 TB/s from L2.  With shorter groups the adding up does: 0.4 us a group of 256
-// rows, half of it the wait for what is read from tensor memory, which 168 registers leave no room to call for ahead.  Scales stay as they are stored
-// until they are used: converted where they are called for, each fourth group waited for memory (81 us with groups of 64).  32 columns of
-// an accumulator at a time instead of 16 do not fit into the registers (90).
+// With groups of 128 x bounds it: 32 KB a step for every SM are 9 TB/s from L2.  With shorter groups the adding up does, whose warps wait for what they
+// read from tensor memory: 176 registers hold 128 sums and 32 columns on their way (16 at a time: 72 and 112).  Scales stay as they are stored until they
+// are used: converted where they were called for, each fourth group waited for memory (81 with groups of 64).  A step with few rows takes 0.45
+// us, by time stamps nearly all of it the issuing lane's waits and commits one after the other; its products are 0.07.
 #include <algorithm>
 #include <type_traits>
 
@@ -50,7 +50,7 @@ constexpr int kAdders = 8, kDecoders = 8;                      // warps
 constexpr int kFirstAdder = 4, kFirstDecoder = kFirstAdder + kAdders;
 constexpr int kThreadsTc = (kFirstDecoder + kDecoders) * 32;
 // Registers: what the CTA starts with is shared out anew, and no more than that.
-constexpr int kStartRegs = 96, kAdderRegs = 168, kOtherRegs = 48;
+constexpr int kStartRegs = 96, kAdderRegs = 176, kOtherRegs = 40;
 static_assert(kAdders * kAdderRegs + (kThreadsTc / 32 - kAdders) * kOtherRegs <= kThreadsTc / 32 * kStartRegs, "more registers than the CTA has");
 constexpr int kPairs = 4;                // pairs of steps whose codes are on their way
 constexpr int kMaxStages = 8, kMaxAccs = 4;
@@ -327,7 +327,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) q4_tc_kernel(const __grid_const
     } else {
         take_registers<kAdderRegs>();
         constexpr int kRows = PARTS == 1 ? 128 : 16;      // of x, that a lane adds up
-        constexpr int kPieces = PARTS == 1 ? kRows / 16 : PARTS;
+        constexpr int kPieces = PARTS == 1 ? kRows / 32 : PARTS;
         const int quarter = warp & 3, half = (warp - kFirstAdder) >> 2;       // of the accumulator's lanes, of the rows of x
         const int rows = PARTS == 1 ? p.tile_rows / 2 : kRows;
         const unsigned from = tmem + ((unsigned)(quarter * 32) << 16) + (unsigned)(half * rows);
@@ -342,22 +342,20 @@ __global__ void __launch_bounds__(kThreadsTc, 1) q4_tc_kernel(const __grid_const
             for (int j = 0; j < kRows / 2; ++j) sum[j] = 0;
             const int first = u.begin * kBK >> p.group_log2, end = ((u.end * kBK - 1) >> p.group_log2) + 1;
             const long long row = min(n, (long long)p.row_tiles * 16 - 1), at = (row >> 4) * p.groups * 16 + (row & 7) * 2 + (row >> 3 & 1);
-            // scales are called for, as they are stored, four groups before they are used; a group behind the last column is all zeros
+            // scales are called for, as they are stored, two groups before they are used; a group behind the last column is all zeros
             auto scale = [&](int q) -> unsigned {
                 if (q >= p.groups) return 0u;
                 const long long o = at + q * 16ll;
                 return p.scale_dtype == DType::F32 ? __ldg((const unsigned*)p.scales + o) : (unsigned)__ldg((const unsigned short*)p.scales + o);
             };
-            unsigned next[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) next[e] = scale(first + e);
-            for (int q = first; q < end && ok; q += 4) {
-                unsigned now[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) now[e] = next[e], next[e] = q + 4 < end ? scale(q + 4 + e) : 0u;
+            unsigned ahead[2] = {scale(first), scale(first + 1)};
 #pragma unroll 1
-                for (int e = 0; e < 4 && q + e < end; ++e) {
-                    const unsigned raw = e == 0 ? now[0] : e == 1 ? now[1] : e == 2 ? now[2] : now[3];
+            for (int q = first; q < end && ok; q += 2) {
+#pragma unroll 1
+                for (int e = 0; e < 2 && q + e < end; ++e) {
+                    const unsigned raw = e == 0 ? ahead[0] : ahead[1];
+                    if (e == 0) ahead[0] = scale(q + 2);
+                    else ahead[1] = scale(q + 3);
                     const float s = p.scale_dtype == DType::F32   ? __uint_as_float(raw)
                                     : p.scale_dtype == DType::F16 ? __half2float(__ushort_as_half((unsigned short)raw))
                                                                   : __uint_as_float(raw << 16);
@@ -367,12 +365,14 @@ __global__ void __launch_bounds__(kThreadsTc, 1) q4_tc_kernel(const __grid_const
                     tc_fence_after();
 #pragma unroll
                     for (int c = 0; c < kPieces; ++c) {
-                        if (PARTS == 1 && c * 16 >= rows) break;
-                        unsigned v[16];
-                        tmem_ld_32x16(from + (unsigned)acc * acc_columns + c * (PARTS == 1 ? 16 : 32), v);
+                        constexpr int W = PARTS == 1 ? 32 : 16;
+                        if (PARTS == 1 && c * W >= rows) break;
+                        unsigned v[W];
+                        if constexpr (PARTS == 1) tmem_ld_32x32(from + (unsigned)acc * acc_columns + c * 32, v);
+                        else tmem_ld_32x16(from + (unsigned)acc * acc_columns + c * 32, v);
                         tmem_ld_wait();
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) add_two(sum[(PARTS == 1 ? c * 8 : 0) + j], v[2 * j], v[2 * j + 1], s2);
+                        for (int j = 0; j < W / 2; ++j) add_two(sum[(PARTS == 1 ? c * W / 2 : 0) + j], v[2 * j], v[2 * j + 1], s2);
                     }
                     tc_fence_before();
                     __syncwarp();
@@ -462,9 +462,9 @@ __global__ void __launch_bounds__(kThreadsTc, 1) q4_tc_kernel(const __grid_const
 // Tiles of few rows of x cost nearly what tiles of many do, as the time goes into the weights' side: so as few waves as 256 rows
 // allow.  The tiles of the last wave are divided along the columns, where the SMs that they leave would wait, if the adding up
 // costs less.  In us: a step of 64 columns takes 0.49 with 64 rows of x and 0.63 with 256 where groups are of 128 columns, 0.03 more where they are
-// shorter, and as long as its groups' adding up where that takes longer (0.74 a group with 256 rows); joining shares 2.5, and 0.007 for each row of x in
+// shorter, and as long as its groups' adding up where that takes longer (0.66 a group with 256 rows); joining shares 2.5, and 0.007 for each row of x in
 // each share.  Rows of f32: 0.50 a step with groups of 128, 0.58 with groups of 64, 0.80 with groups of 32.  Estimated / measured, f16: 11008 x 4096,
-// groups of 128, 9 / 64 / 500 rows 34.5 / 38.0, 36.6 / 38.4, 65 / 62; 4096 x 11008, groups of 64, 64 / 500 rows 33 / 34, 78 / 75.
+// groups of 128, 9 / 64 / 500 rows 34.5 / 38.0, 36.6 / 38.4, 65 / 62; 4096 x 11008, groups of 64, 64 / 500 rows 33 / 34, 71 / 68.
 Q4TcPlan q4_tc_plan(Device& dev, const Q4Weight& w, int64_t rows, int parts) {
     Q4TcPlan best;
     const bool split = parts > 1;
@@ -476,7 +476,7 @@ Q4TcPlan q4_tc_plan(Device& dev, const Q4Weight& w, int64_t rows, int parts) {
         before = tile_rows;
         const int64_t tiles = tiles_n * ((rows + tile_rows - 1) / tile_rows), whole = tiles / sms * sms, rest = tiles - whole;
         const double step = split ? (w.group == 32 ? 0.80 : w.group == 64 ? 0.58 : 0.50)
-                                  : std::max((w.group == 128 ? 0.45 : 0.48) + 0.0007 * (double)tile_rows, (0.10 + 0.0025 * (double)tile_rows) * 64.0 / (double)w.group);
+                                  : std::max((w.group == 128 ? 0.45 : 0.48) + 0.0007 * (double)tile_rows, (0.10 + 0.0022 * (double)tile_rows) * 64.0 / (double)w.group);
         const double start = 5.0 + (double)(whole / sms * w.chunks) * step;
         const int most = rest ? (int)std::min<int64_t>(sms / rest, 32) : 1;      // a CTA has one share at most
         for (int s = 1; s <= most; ++s) {
