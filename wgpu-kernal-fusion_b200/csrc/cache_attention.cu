@@ -5,8 +5,8 @@
 //
 // What bounds it: every key and value of the cache is read once, 2 * head_dim bytes a token and kv head, for at most
 // a few rows, so it is memory.  The product is done by the warps' own m16n8k16 instructions: their B operand comes
-// from registers, which is where the codes are after the conversion to f16, while the fifth-generation instructions
-// would want the converted operand in shared memory, twice the cache's bytes written and read there.
+// from registers, which is where the codes are after the conversion to f16.  The fifth-generation instructions take operands from
+// shared and tensor memory, where every converted code would have to be written first, for eight rows that use it.
 //   * A warp works on a block of 64 tokens by itself: running maximum, sum and accumulator in registers, no
 //     barrier anywhere in the loop.  The cache is stored in the order in which lanes want it (kv_cache.cu), so a lane
 //     copies the bytes that it will read itself (16 at a time, asynchronously, three half blocks in flight).
@@ -22,9 +22,9 @@
 //     a CTA), and every CTA takes an equal stretch of it, as the kernel itself computes from the lengths: ragged
 //     batches are even, and a recorded launch stays even while its sequences grow.  The last CTA to finish a job
 //     that several have a stretch of joins their parts, in their order, so results do not depend on timing.
-// One token over 131071 of 8 kv heads, 269 MB: the CTAs' loops take 42 us (6.4 TB/s of the measured 6.56), a pass 55 us with
+// One token over 131071 of 8 kv heads, 269 MB: the CTAs' loops take 42 us (6.4 TB/s of the measured 6.56), a pass 55 to 57 us by card with
 // the launch, the first loads and the joining; with two half blocks in a ring instead of three it took 87.  32 sequences of up to
-// 8192 tokens, 310 MB: 75 us, 84 where each job had a number of CTAs of its own.
+// 8192 tokens, 310 MB: 74 to 76 us, 84 where each job had a number of CTAs of its own.
 #include <algorithm>
 
 #include "decode.hpp"

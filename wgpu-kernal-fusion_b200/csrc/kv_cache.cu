@@ -17,7 +17,7 @@
 // in shared memory (old ones from the tail, new ones from the call, keys behind norm and rotation if asked), finds the
 // largest magnitude on the way and writes the codes; for long prompts it is bound by memory, for one token by
 // the latency of one load, one reduction and one store.
-// 4 sequences of up to 2048 tokens, 8 heads of 128, bf16, 79 MB in and out: an append into an emptied cache and a read of it take 36 us,
+// 4 sequences of up to 2048 tokens, 8 heads of 128, bf16, 79 MB in and out: an append into an emptied cache and a read of it take 36 to 37 us,
 // 20 in the append kernel and 13 in the read, both bound by the instructions that turn values into codes and into the lanes' order
 // (about 30 a value) and back, not by memory, which would need 12 for both.
 #include <algorithm>

@@ -14,13 +14,12 @@
 // bound, and next to it the instructions that turn words into operands (about 80 of f16 and 85 of bf16 for the 16 x 64 weights of a
 // unit; 11008 x 4096 weights are 74 units for each scheduler of the GPU).  The instruction's eight columns are the
 // rows of x; codes become f16 or bf16 exactly, and sums are f32 within a group and across groups.  A row of f32 takes
-// three columns: its bf16 parts, which together have its 24 bits.  The product does not go through tensor memory: for
-// eight columns a tile of 128 rows would have to be converted into shared memory first, and the conversion, not the
-// product, is the work here.
-// One row through 11008 x 4096, groups of 128, f16, recorded: 10.3 us a pass (23 MB; 7 of them in the kernel, 3.5 at the
-// measured rate of memory); 16.5 with a CTA for each row tile, whose first loads, staging of x and sums were not
+// three columns: its bf16 parts, which together have its 24 bits.  The product does not go through tensor memory: the
+// converted codes would have to be written there, or to shared memory, first, and for eight columns the conversion, not the product, is the work.
+// One row through 11008 x 4096, groups of 128, f16, recorded: 10.7 to 12.3 us a pass (such passes come in steps of 2.05), 10.5 in a row of
+// products (23 MB; 3.5 at the measured rate of memory); 16.5 with a CTA for each row tile, whose first loads, staging of x and sums were not
 // overlapped with anything, and 22 where a scale was converted, and so waited for, in the turn that called for it.
-// Seven rows of bf16 through 4096 x 11008: 14.4 us.
+// Seven rows of bf16 through 4096 x 11008: 14.7 us a pass, 13 in a row of products.
 // More rows: in blocks, along the grid's second axis, or on the tensor cores (q4_tc.cu; choose_way has the times).
 #include <algorithm>
 

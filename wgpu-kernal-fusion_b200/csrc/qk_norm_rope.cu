@@ -8,7 +8,7 @@
 // second being the rotation's partner of the first), so the mean needs three shuffles and no shared memory.
 // A group takes HEADS heads of one token: their loads are all issued before the first is used, and the products of
 // weights with cosines and sines are made once for them.
-// 8 x 2048 tokens of 32 + 8 heads of 128, f16, 336 MB: 61.5 us (5.5 TB/s, 0.83 of the measured copy); with blocks of 256
+// 8 x 2048 tokens of 32 + 8 heads of 128, f16, 336 MB: 61.5 to 65.7 us by card (5.1 to 5.5 TB/s, 0.78 to 0.83 of the measured copy); with blocks of 256
 // threads 70, with two heads a group 72 to 102, and 118 where rows were turned into f32 as they came (twice the registers).
 #include <algorithm>
 
