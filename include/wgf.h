@@ -388,7 +388,8 @@ int32_t wgf_q4_weight_info(wgf_q4_weight* w, int64_t* n, int64_t* k, uint32_t* g
 int32_t wgf_q4_weight_dequantize(wgf_q4_weight* w, uint32_t dtype, wgf_tensor** out);
 /* x [.., k] times the transposed weights: [.., n] of x's type, lazily, in one kernel (two for many rows of f32, or of
  * 16 bits that do not begin at 16-byte borders).  f32 sums of exact products for any number of rows and every type: the
- * weights' values are rounded nowhere on the way, and the result once. */
+ * weights' values are rounded nowhere on the way, and the result once.  (A row of f32 goes as three bf16 parts:
+ * what of it is below 2^-133 falls away, so values below 2^-110 lose digits.) */
 int32_t wgf_tensor_matmul_q4(wgf_tensor* x, wgf_q4_weight* w, wgf_tensor** out);
 
 /* ======================================================================================

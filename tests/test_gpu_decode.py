@@ -962,3 +962,18 @@ def test_cache_of_the_largest_numbers_is_finite(kind, sign, wgf, dev):
     one.append(give(wgf, dev, x[:, :, 3:4] * 0, kind), give(wgf, dev, x[:, :, 3:4], kind))
     out = take(one.attention(give(wgf, dev, x[:, :, :1], kind)), kind)
     np.testing.assert_array_equal(out[0, 0, 0], ref.round_to(ref.stands_for(x[0, 0, 3:4]), kind)[0])
+
+
+@pytest.mark.parametrize("kind,exponent", [("f32", -107), ("bf16", -120), ("f16", -18), ("f32", 90), ("bf16", 90)])
+@pytest.mark.parametrize("rows,n,k", [(3, 40, 256), (300, 1100, 1100)])
+def test_q4_product_of_far_sizes_of_x(kind, exponent, rows, n, k, wgf, dev):
+    """Small and large rows keep the bound that ordinary ones have, with scales that bring the result back."""
+    g = seeded(32, rows - exponent)
+    c = g.integers(-8, 8, (n, k))
+    s = np.full((n, -(-k // 64)), 2.0 ** (20 if exponent < 0 else -40), np.float32)
+    x = ref.round_to(g.standard_normal((rows, k)) * 2.0 ** exponent, kind)
+    out = take(give(wgf, dev, x, kind).mat_mul_q4(from_codes(wgf, dev, c, s, 64)), kind)
+    want, bound = ref.q4_product(x, ref.q4_values(c, s, 64), kind)
+    # denormal numbers: f16 has steps of 2^-24 there, which are exact; of an f32 value half a step of its third part, 2^-134, may be missing
+    lost = 2.0 ** -134 * np.abs(ref.q4_values(c, s, 64)).sum(1)[None] if kind == "f32" else 0.0
+    close(out, want, bound + lost)
